@@ -1,0 +1,40 @@
+// Launch struct of the normalised sum (add_norm.hip); beside the C ABI, for the extension.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <stddef.h>
+
+namespace dcn {
+
+// A matrix of rows: its type's code and the elements between rows; rows need only their elements' alignment.
+struct NormRows {
+  const void *base;
+  int dtype;
+  long long pitch;
+};
+
+// out = LayerNorm(x + residual) over rows of `width`, and the sum itself.
+struct AddNormLaunch {
+  NormRows x, residual;           // residual may be null; of x's type or fp32
+  const void *weight, *bias;      // of type param_dtype, or null: ones and zeros
+  int param_dtype;
+  long long rows;
+  int width;
+  float eps;
+  void *out, *sum;                // dense; the sum may be null
+  int out_dtype, sum_dtype;
+  float *stats;                   // (rows, 2): mean and 1 / deviation; the forward writes them where they are wanted
+  // backward: x and residual (or the sum, as x), stats, and
+  const void *grad_out, *grad_sum;                  // dense, of the outputs' types; grad_sum may be null
+  void *grad_x, *grad_residual;                     // dense; grad_residual may be null
+  int grad_x_dtype, grad_residual_dtype;
+  void *grad_weight, *grad_bias;                    // each may be null
+  void *workspace;
+};
+
+constexpr int kMaxNormWidth = 8192;
+size_t add_norm_backward_workspace_bytes(const AddNormLaunch &p);
+hipError_t launch_add_norm_forward(const AddNormLaunch &p, hipStream_t stream);
+hipError_t launch_add_norm_backward(const AddNormLaunch &p, hipStream_t stream);
+
+}  // namespace dcn

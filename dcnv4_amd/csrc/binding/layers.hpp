@@ -75,5 +75,6 @@ void weight_gradients(int code, const at::TensorOptions &fp32, const std::vector
 extern PyMethodDef training_methods[];
 extern PyMethodDef attention_methods[];
 extern PyMethodDef convolution_methods[];
+extern PyMethodDef decoder_methods[];
 
 }  // namespace dcn::binding

@@ -1,0 +1,38 @@
+// Launch struct of the attention among queries (query_attention.hip); beside the C ABI, for the extension.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <stddef.h>
+
+namespace dcn {
+
+// A (batch, tokens, heads, width) tensor: elements between neighbours; the width is dense, its rows start on 16 bytes.
+struct AttnRows {
+  const void *base;
+  long long batch, token, head;
+};
+
+struct AttnLaunch {
+  AttnRows q, k, v;
+  int batch, nq, nk, heads, kv_heads, width;      // width: a multiple of 8, at most kMaxAttnWidth
+  float scale, cap;                               // cap 0: scores as they are
+  const int *q_segments, *k_segments;             // (batch, tokens); no k_segments: all see all; no q_segments: zeros
+  const float *q_points, *k_points, *slopes;      // (batch, tokens, 2), (heads,): all or none
+  void *out;                                      // dense (batch, nq, heads, width)
+  float *lse;                                     // (batch, heads, nq): log of a row's sum; infinite where it sees nothing
+  // backward; gradients are dense and of the tensors' type
+  AttnRows grad_out;
+  void *grad_q, *grad_k, *grad_v;                 // null where not wanted
+  float *grad_slopes;                             // (heads,) or null
+  void *workspace;
+};
+
+constexpr int kMaxAttnWidth = 128;
+// Scratch of a call, 256-byte aligned; destroyed.
+size_t attn_forward_workspace_bytes(int dtype, const AttnLaunch &p);
+size_t attn_backward_workspace_bytes(int dtype, const AttnLaunch &p);
+hipError_t launch_attn_forward(int dtype, const AttnLaunch &p, hipStream_t stream);
+// Wants out and lse of the forward.
+hipError_t launch_attn_backward(int dtype, const AttnLaunch &p, hipStream_t stream);
+
+}  // namespace dcn

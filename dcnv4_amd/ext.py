@@ -328,6 +328,32 @@ def flash_deform_attn_backward_split(value, spatial_shapes, level_start_index, s
                                               grad_output, im2col_step, K, d_stride, block_thread)
 
 
+def query_attention_forward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap):
+    """``[output, lse]`` of :func:`dcnv4_amd.functions.query_attention`, nothing left out: ``key_segments`` beside ``segments``,
+    positions of both beside ``slopes``; each of the five may be None.  ``lse`` (N, M, Lq) float32: the logarithm of a row's sum
+    of exponentials, infinite for a row that sees nothing."""
+    return _native.query_attention_forward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap)
+
+
+def query_attention_backward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap, output, lse,
+                             grad_output):
+    """``[grad_query, grad_key, grad_value, grad_slopes]`` of :func:`query_attention_forward`; the last None without slopes."""
+    return _native.query_attention_backward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap,
+                                            output, lse, grad_output)
+
+
+def add_layer_norm_forward(input, residual, weight, bias, eps, wide=False):
+    """``[output, sum, stats]``: ``layer_norm(input + residual)`` over the last axis, the sum, and (rows, 2) float32 means and
+    inverse deviations.  ``residual``, ``weight`` and ``bias`` may be None; ``wide``: a float32 result whatever the inputs."""
+    return _native.add_layer_norm_forward(input, residual, weight, bias, eps, wide)
+
+
+def add_layer_norm_backward(input, residual, weight, bias, eps, wide, stats, grad_output, grad_sum=None):
+    """``[grad_input, grad_residual, grad_weight, grad_bias]`` of :func:`add_layer_norm_forward`, None for what is absent;
+    ``grad_sum`` is the gradient that reaches the sum itself."""
+    return _native.add_layer_norm_backward(input, residual, weight, bias, eps, wide, stats, grad_output, grad_sum)
+
+
 def stream_copy(src, dst):
     """Copies ``src`` into ``dst`` (same byte size, a multiple of 16) with the library's streaming kernel: the measured
     memory ceiling of the benchmark and the known-size workload that calibrates byte counters."""
