@@ -49,6 +49,7 @@ AttnShape attn_check(const AttnInputs &a) {
     raise_runtime("%lld heads of the query do not share %lld heads of the key evenly", (long long)s.heads, (long long)s.kv_heads);
   if (s.width < 1 || s.width > kMaxAttnWidth) raise_runtime("heads of %lld channels are not supported (1 to %d)", (long long)s.width, kMaxAttnWidth);
   // rows are counted in 32 bits by the kernels
+  if (s.nq > (1 << 30) || s.nk > (1 << 30)) raise_runtime("sequences of more than 2^30 tokens");
   if (s.batch * s.nq * s.heads > kIntMax || s.batch * s.nk * s.kv_heads > kIntMax) raise_runtime("more than 2^31 - 1 rows of queries or keys");
   if (!(a.scale == a.scale) || !(a.cap >= 0.f) || a.cap > 3e38f) raise_runtime("cap must be zero (none) or positive and finite, scale a number");
   if (a.q_segments.defined()) {
@@ -99,29 +100,35 @@ struct AttnCall {
   }
 };
 
-// {out, lse}; lse (batch, heads, queries) only where it is wanted
-std::pair<Tensor, Tensor> attn_forward(const AttnInputs &a, bool want_lse) {
+// What the backward needs of a forward: the result, what rounding took from it (16-bit types) and (batch, heads, queries) logarithms.
+struct AttnOutputs {
+  Tensor out, rest, lse;
+};
+AttnOutputs attn_forward(const AttnInputs &a, bool train) {
   const AttnShape s = attn_check(a);
   OnDevice guard(a.q);
-  Tensor out = at::empty({s.batch, s.nq, s.heads, s.padded()}, a.q.options()), lse;
-  if (want_lse) lse = at::empty({s.batch, s.heads, s.nq}, a.q.options().dtype(at::kFloat));
+  Tensor out = at::empty({s.batch, s.nq, s.heads, s.padded()}, a.q.options()), rest, lse;
+  if (train) lse = at::empty({s.batch, s.heads, s.nq}, a.q.options().dtype(at::kFloat));
+  if (train && s.code != DCNV4_DTYPE_F32) rest = at::empty(out.sizes(), out.options());
   if (out.numel() != 0) {
     AttnCall c(a, s);
     c.l.out = out.data_ptr();
+    c.l.out_rest = ptr(rest);
     c.l.lse = static_cast<float *>(ptr(lse));
     const Tensor ws = workspace(attn_forward_workspace_bytes(s.code, c.l), a.q);
     c.l.workspace = ptr(ws);
     hip_check(launch_attn_forward(s.code, c.l, static_cast<hipStream_t>(stream_of(a.q))), "query_attention");
   }
-  return {narrowed(out, s), lse};
+  return {narrowed(out, s), rest.defined() ? narrowed(rest, s) : rest, lse};
 }
 
 // Gradients of query, key, value and slopes, those that are wanted.
-std::array<Tensor, 4> attn_backward(const AttnInputs &a, const Tensor &out, const Tensor &lse, const Tensor &grad_out, std::array<bool, 4> want) {
+std::array<Tensor, 4> attn_backward(const AttnInputs &a, const AttnOutputs &found, const Tensor &grad_out, std::array<bool, 4> want) {
   const AttnShape s = attn_check(a);
   check_beside(grad_out, "grad_output", a.q, a.q.scalar_type(), a.q.sizes());
-  check_beside(out, "output", a.q, a.q.scalar_type(), a.q.sizes());
-  check_beside(lse, "lse", a.q, at::kFloat, {s.batch, s.heads, s.nq});
+  check_beside(found.out, "output", a.q, a.q.scalar_type(), a.q.sizes());
+  if (found.rest.defined()) check_beside(found.rest, "rest", a.q, a.q.scalar_type(), a.q.sizes());
+  check_beside(found.lse, "lse", a.q, at::kFloat, {s.batch, s.heads, s.nq});
   OnDevice guard(a.q);
   std::array<Tensor, 4> grads;
   const auto options = a.q.options();
@@ -133,8 +140,10 @@ std::array<Tensor, 4> attn_backward(const AttnInputs &a, const Tensor &out, cons
   if (want[3] && a.slopes.defined()) grads[3] = make({s.heads}, a.slopes.options());
   if (!empty) {
     AttnCall c(a, s);
-    const Tensor o = attn_rows(out, s).contiguous(), g = attn_rows(grad_out, s), l = lse.contiguous();
+    const Tensor o = attn_rows(found.out, s).contiguous(), r = found.rest.defined() ? attn_rows(found.rest, s).contiguous() : found.rest;
+    const Tensor g = attn_rows(grad_out, s), l = found.lse.contiguous();
     c.l.out = o.data_ptr();
+    c.l.out_rest = ptr(r);
     c.l.lse = l.data_ptr<float>();
     c.l.grad_out = row_view(g);
     c.l.grad_q = ptr(grads[0]); c.l.grad_k = ptr(grads[1]); c.l.grad_v = ptr(grads[2]);
@@ -150,7 +159,7 @@ std::array<Tensor, 4> attn_backward(const AttnInputs &a, const Tensor &out, cons
 
 struct QueryAttentionBackward final : torch::autograd::Node {
   SavedVariable q, k, v, q_segments, k_segments, q_points, k_points, slopes, out;
-  Tensor lse;
+  Tensor rest, lse;
   float scale, cap;
 
   explicit QueryAttentionBackward(const AttnInputs &a)
@@ -159,7 +168,7 @@ struct QueryAttentionBackward final : torch::autograd::Node {
   std::string name() const override { return "QueryAttentionFunctionBackward"; }
   void release_variables() override {
     for (SavedVariable *s : {&q, &k, &v, &q_segments, &k_segments, &q_points, &k_points, &slopes, &out}) s->reset_data();
-    lse = Tensor();
+    rest = lse = Tensor();
   }
   variable_list apply(variable_list &&grads) override {
     if (!grads[0].defined()) return variable_list(4);
@@ -170,7 +179,7 @@ struct QueryAttentionBackward final : torch::autograd::Node {
                             slopes.unpack(), scale, cap};
       const Tensor o = out.unpack(shared_from_this());
       Tensor g = grads[0]._is_zerotensor() ? at::zeros(grads[0].sizes(), grads[0].options()) : grads[0];
-      got = attn_backward(a, o, lse, g, {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2),
+      got = attn_backward(a, {o, rest, lse}, g, {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2),
                                          task_should_compute_output(3)});
     }
     return once_differentiable({got[0], got[1], got[2], got[3]});
@@ -203,28 +212,18 @@ PyObject *py_query_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     const bool train = wants_grad({&in.q, &in.k, &in.v, &in.slopes});
-    Tensor lse;
-    std::tie(out, lse) = attn_forward(in, train);
+    AttnOutputs found = attn_forward(in, train);
+    out = found.out;
     if (train) {
       std::shared_ptr<QueryAttentionBackward> node(new QueryAttentionBackward(in), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(in.q, in.k, in.v, in.slopes));
       record(node, out);
       node->out = SavedVariable(out, true);
-      node->lse = lse;
+      node->rest = found.rest;
+      node->lse = found.lse;
     }
   }
   return THPVariable_Wrap(std::move(out));
-  END_HANDLE_TH_ERRORS
-}
-
-// The arguments above: [out, lse]
-PyObject *py_query_attention_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  Args a("query_attention_forward", args, n, 10);
-  const AttnInputs in = attn_inputs(a);
-  at::AutoGradMode no_grad(false);
-  auto r = attn_forward(in, true);
-  return Py_BuildValue("[NN]", THPVariable_Wrap(r.first), THPVariable_Wrap(r.second));
   END_HANDLE_TH_ERRORS
 }
 
@@ -233,14 +232,29 @@ PyObject *wrapped(const Tensor &t) {
   Py_RETURN_NONE;
 }
 
-// The arguments above, out, lse, grad_output: [grad_query, grad_key, grad_value, grad_slopes or None]
+// The arguments above: [out, rest or None, lse]
+PyObject *py_query_attention_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("query_attention_forward", args, n, 10);
+  const AttnInputs in = attn_inputs(a);
+  at::AutoGradMode no_grad(false);
+  const AttnOutputs r = attn_forward(in, true);
+  return Py_BuildValue("[NNN]", wrapped(r.out), wrapped(r.rest), wrapped(r.lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// The arguments above, out, rest or None, lse, grad_output: [grad_query, grad_key, grad_value, grad_slopes or None]
 PyObject *py_query_attention_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  Args a("query_attention_backward", args, n, 13);
+  Args a("query_attention_backward", args, n, 14);
   const AttnInputs in = attn_inputs(a);
-  const Tensor &out = a.tensor(), &lse = a.tensor(), &grad = a.tensor();
+  AttnOutputs found;
+  found.out = a.tensor();
+  found.rest = a.optional_tensor();
+  found.lse = a.tensor();
+  const Tensor &grad = a.tensor();
   at::AutoGradMode no_grad(false);
-  const auto g = attn_backward(in, out, lse, grad, {true, true, true, true});
+  const auto g = attn_backward(in, found, grad, {true, true, true, true});
   return Py_BuildValue("[NNNN]", wrapped(g[0]), wrapped(g[1]), wrapped(g[2]), wrapped(g[3]));
   END_HANDLE_TH_ERRORS
 }

@@ -5,252 +5,1194 @@
 //   dV = P^T dO,  dS = P (dO V^T - delta),  dslope = -sum dS |p_i - p_j|,  dX = dS (1 - tanh^2),  dQ = scale dX K,  dK = scale dX^T Q
 // Heads that share a key head add up in its gradient.
 //
-// A wave owns a row: of 64 keys at a time (queries, for the gradients of a key) each lane forms the score of its own, the
-// lanes then take a column of the result each and walk the 64.  What a row does not see is skipped, not multiplied by zero, so
-// infinities and NaN there go nowhere.
+// One scheme for the three kernels (forward, dQ, dK and dV).  A workgroup owns *columns* - queries, queries, keys - whose operands
+// lie in registers, and walks *rows* - keys, keys, queries - in tiles that come through LDS.  A matrix instruction forms 16 rows x 16
+// columns of scores with the rows first: lane (g, c) then holds rows 4 g .. + 3 of column c, which is how the next instruction
+// wants the weights, as its second operand with the rows as depth, so weights never leave the registers.  Its first operand is
+// the tile again with rows and width exchanged: 16-bit types are turned by the transposing LDS read, fp32 needs one element a lane.
+// Everything that belongs to a column (maximum, sum, logarithm, delta, scales) is one register a lane.
+//
+// The scores of a tile are 16 instructions' issue slots or more a lane against few matrix clocks at widths of 32 and 64, so it is the
+// vector instructions that are counted there: the running maximum moves only when a score passes it by 2^8, and the row sums of 16-bit
+// types are a product with ones.
 #include "query_attention.hpp"
 
+#include <algorithm>
+
 #include "common.hpp"
+#include "launch.hpp"
 #include "mfma.hpp"
 
 namespace dcn {
 namespace {
 
-constexpr int kRowThreads = 256, kRowWaves = kRowThreads / kWave;
-constexpr float kInf = __builtin_inff();
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr float kInf = __builtin_inff(), kLog2e = 1.44269504088896340736f;
+constexpr int kHiddenColumn = -2;      // the segment of a column or query row that sees nothing; -1 is a padded key's
 
-__device__ __forceinline__ float wave_max(float v) {
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
-  return v;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Rounding of P and dX to fp16 next to its subnormals would cost what bf16 and fp32 never lose: exponents are moved up, and
+// back in the results.  Forward: weights against a maximum that is up to 2^8 behind stay below 2^12.
+template <typename Tag> constexpr float kForwardShift = Tag::kCode == F16::kCode ? 4.f : 0.f;
+// Backward: weights of at most 1; a row of a million keys still has normal ones.
+template <typename Tag> constexpr float kBackwardShift = Tag::kCode == F16::kCode ? 12.f : 0.f;
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// Over the four lanes that share a column.
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, kWave));
+  return fmaxf(v, __shfl_xor(v, 32, kWave));
 }
-__device__ __forceinline__ float wave_sum(float v) { return cluster_sum(v, kWave); }
-
-template <typename Tag>
-__device__ __forceinline__ const char *row_of(const AttnRows &t, int b, int token, int head) {
-  return static_cast<const char *>(t.base) + (b * t.batch + token * t.token + head * t.head) * (long long)Tag::kBytes;
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16, kWave);
+  return v + __shfl_xor(v, 32, kWave);
 }
 
-// Dot product of a row in memory with one in LDS.
+// A kernel's shape.  W: the width, zeros behind the tensors' own; RT: rows of a tile; RW: waves that share the columns and divide
+// a tile's rows, the others divide the columns; CF: sixteens of columns a wave.
+template <typename Tag_, int W_, int RT_, int RW_, int CF_>
+struct Shape {
+  typedef Tag_ Tag;
+  static constexpr int W = W_, RT = RT_, RW = RW_, CF = CF_;
+  static constexpr int kSlices = W * Tag::kBytes / 64, kWidthBlocks = W / 16;
+  static constexpr int kColumnWaves = kWaves / RW, kColumns = 16 * CF * kColumnWaves;
+  static constexpr int kRowBlocks = RT / RW / 16;                // of a wave in a tile
+  static constexpr int kTensorBytes = RT * W * Tag::kBytes;
+  // two tensors, then by row: segment, poison, position (2), logarithm, delta
+  static constexpr int kSegments = 2 * kTensorBytes, kPoison = kSegments + RT * 4, kPoints = kPoison + RT * 4, kLse = kPoints + RT * 8,
+                       kDelta = kLse + RT * 4, kTileBytes = kDelta + RT * 4;
+  static constexpr int kMergeBytes = RW > 1 ? kWaves * 16 * CF * (W + 4) * 4 + kWaves * 16 * CF * 8 : 0;
+  static constexpr int kLdsBytes = std::max(2 * kTileBytes, kMergeBytes);
+  static_assert(kRowBlocks % 2 == 0 && kLdsBytes <= 156 * 1024);
+};
+
+// ---------------------------------------------------------------- a tile's way into LDS
+// Rows in slices of 64 bytes, 16 to a block of 1 KB, a row's vectors at vector ^ (row / 4 & 3) (fragment_offset): both the fragment
+// reads and the transposing ones then spread over the banks.  A wave carries sixteens of rows, four lanes a row.
+__device__ __forceinline__ uint32_t fragment_at(int r16, int kb) { return (uint32_t)(r16 * 64 + (kb ^ ((r16 >> 2) & 3)) * 16); }
+
+struct HeadRows {
+  const char *base;
+  long long pitch;      // bytes
+};
 template <typename Tag>
-__device__ __forceinline__ float dot_row(const char *row, const float *other, int width) {
-  float sum = 0.f;
-  for (int d = 0; d < width; d += 8) {
-    float f[8];
-    load8<Tag>(row, d, f);
+__device__ __forceinline__ HeadRows head_rows(const AttnRows &t, int b, int head) {
+  return {static_cast<const char *>(t.base) + (b * t.batch + head * t.head) * (long long)Tag::kBytes, t.token * (long long)Tag::kBytes};
+}
+
+template <typename S>
+struct TileLoads {
+  u32x4 v[S::RT / 64][S::kSlices];
+
+  __device__ __forceinline__ void request(const HeadRows &t, int row0, int rows, int width_bytes, int wave, int lane) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(t.base + row0 * t.pitch, 0x7fffffffu);
+    const int vec = (lane & 3) ^ ((lane >> 4) & 3);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) sum = fmaf(f[c], other[d + c], sum);
+    for (int u = 0; u < S::RT / 64; ++u) {
+      const int row = (wave + 4 * u) * 16 + lane / 4;
+      const uint32_t at = (uint32_t)row * (uint32_t)t.pitch + (uint32_t)vec * 16;
+#pragma unroll
+      for (int s = 0; s < S::kSlices; ++s)
+        v[u][s] = buffer_load<16>(r, row0 + row < rows && s * 64 + vec * 16 < width_bytes ? at + s * 64 : kDropOffset);
+    }
   }
+  __device__ __forceinline__ void put(char *tensor, int wave, int lane) const {
+#pragma unroll
+    for (int u = 0; u < S::RT / 64; ++u)
+#pragma unroll
+      for (int s = 0; s < S::kSlices; ++s)
+        *reinterpret_cast<u32x4 *>(tensor + s * S::RT * 64 + (wave + 4 * u) * 1024 + lane * 16) = v[u][s];
+  }
+  // Clears vectors that hold an infinity or NaN; whether the lane's row u had one.
+  __device__ __forceinline__ bool clear_bad(int u) {
+    constexpr uint32_t top = S::Tag::kCode == F32::kCode ? 0x7f800000u : S::Tag::kCode == F16::kCode ? 0x7c00u : 0x7f80u;
+    bool row = false;
+#pragma unroll
+    for (int s = 0; s < S::kSlices; ++s) {
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bad = bad || (v[u][s][i] & top) == top;
+        if constexpr (S::Tag::kBytes == 2) bad = bad || (v[u][s][i] & top << 16) == top << 16;
+      }
+      if (bad) v[u][s] = u32x4{0, 0, 0, 0};
+      row = row || bad;
+    }
+    return row;
+  }
+};
+// A row that holds an infinity or NaN, in a tile of which some columns do not see all: zeros in the products (0 times either would
+// reach every column), and this added to its scores, so that the columns that do see it get NaN.
+template <typename S>
+__device__ __forceinline__ void put_poison(char *tile, int u, bool bad, int wave, int lane) {
+  const uint64_t all = __ballot(bad);
+  if ((lane & 3) == 0)
+    reinterpret_cast<float *>(tile + S::kPoison)[(wave + 4 * u) * 16 + lane / 4] = (all >> lane & 15) != 0 ? __builtin_nanf("") : 0.f;
+}
+
+template <typename S>
+__device__ __forceinline__ u32x4 fragment(const char *tensor, int block, int slice, int lane) {
+  return *reinterpret_cast<const u32x4 *>(tensor + slice * S::RT * 64 + block * 1024 + fragment_at(lane & 15, lane >> 4));
+}
+// acc[d][f] += rows 16 block .. + 31 of the tensor, turned, times the weights in p[0], p[1]
+template <typename S>
+__device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF], const char *tensor, int block, const f32x4 (&p)[2][S::CF], int lane) {
+  typedef typename S::Tag Tag;
+  const int g = lane >> 4, c = lane & 15;
+  if constexpr (Tag::kBytes == 2) {
+    u32x4 w[S::CF];
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      const float v[8] = {p[0][f].x, p[0][f].y, p[0][f].z, p[0][f].w, p[1][f].x, p[1][f].y, p[1][f].z, p[1][f].w};
+      w[f] = Pack<Tag, 8>::encode(v);
+    }
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) {
+      const char *at = tensor + d / 2 * S::RT * 64 + block * 1024 + (4 * g + (c >> 2)) * 64 + (((d & 1) * 2 + ((c & 3) >> 1)) ^ g) * 16 + (c & 1) * 8;
+      typedef __attribute__((address_space(3))) s16x4 lds_words;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_words *)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_words *)(at + 1024));
+      const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+      const u32x4 turned = {a.x, a.y, b.x, b.y};
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) acc[d][f] = mfma_64_bytes<Tag>(turned, w[f], acc[d][f]);
+    }
+  } else {
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const char *at = tensor + d * S::RT * 64 + (block + half) * 1024 + 4 * g * 64 + ((c >> 2) ^ g) * 16 + (c & 3) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float a = *reinterpret_cast<const float *>(at + r * 64);
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) acc[d][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[half][f][r], acc[d][f], 0, 0, 0);
+        }
+      }
+  }
+}
+
+// A column's operand, straight from memory: the second operand of the score products.
+template <typename S>
+__device__ __forceinline__ void load_columns(u32x4 (&to)[S::CF][S::kSlices], const HeadRows &t, int column0, int columns, int width_bytes, int lane) {
+  const __amdgpu_buffer_rsrc_t r = make_rsrc(t.base + column0 * t.pitch, 0x7fffffffu);
+  const int kb = lane >> 4;
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const int column = 16 * f + (lane & 15);
+#pragma unroll
+    for (int s = 0; s < S::kSlices; ++s)
+      to[f][s] = buffer_load<16>(r, column0 + column < columns && s * 64 + kb * 16 < width_bytes ? (uint32_t)column * (uint32_t)t.pitch + s * 64 + kb * 16 : kDropOffset);
+  }
+}
+template <typename Tag>
+__device__ __forceinline__ float dot_16_bytes(u32x4 a, u32x4 b, float sum) {
+  constexpr int N = 16 / Tag::kBytes;
+  float x[N], y[N];
+  Pack<Tag, N>::decode(a, x);
+  Pack<Tag, N>::decode(b, y);
+#pragma unroll
+  for (int i = 0; i < N; ++i) sum = fmaf(x[i], y[i], sum);
   return sum;
 }
 
-struct Score {
-  float s, slope_factor, bent;      // the score; the distance; 1 - tanh^2
+// ---------------------------------------------------------------- scores
+// Scores go into exp2, so they are in units of its exponent.  Without cap and distance that is one factor, which rides along where
+// the maximum is taken off.
+struct Scores {
+  float cap, scale, tanh_scale, factor, slope;
+  bool bent, apart;      // there is a cap; a distance
+  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : cap(p.cap), scale(p.scale), bent(p.cap > 0.f), apart(p.slopes != nullptr) {
+    tanh_scale = bent ? scale / cap : 0.f;
+    factor = (bent ? cap : scale) * kLog2e;
+    slope = apart ? p.slopes[head] * kLog2e : 0.f;
+  }
+  // the products as they come may stand for the scores, in the order of their size
+  __device__ __forceinline__ bool as_they_are() const { return !bent && !apart && scale > 0.f; }
+  template <typename Tag>
+  __device__ __forceinline__ float tanh_of(float product) const {
+    const float x = product * tanh_scale;
+    if constexpr (Tag::kBytes == 4) return tanhf(x);      // fp32 results see the last bits
+    else return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e)) + 1.f), 1.f);
+  }
 };
-__device__ __forceinline__ Score finish_score(const AttnLaunch &p, float dot, int b, int head, int i, int j) {
-  Score r;
-  r.s = dot * p.scale;
-  r.bent = 1.f;
-  if (p.cap > 0.f) {
-    const float t = tanhf(r.s / p.cap);
-    r.s = p.cap * t;
-    r.bent = fmaf(-t, t, 1.f);
+__device__ __forceinline__ float distance(f32x2 a, f32x2 b) {
+  const float x = a.x - b.x, y = a.y - b.y;
+  return __builtin_amdgcn_sqrtf(fmaf(x, x, y * y));
+}
+
+// ---------------------------------------------------------------- which tiles
+// What the segment numbers of a workgroup's columns leave of a tile: whether any pair sees each other and whether all do.
+struct ColumnRange {
+  int lo, hi;              // of the numbers that count
+  bool shared, hidden;     // a key column of segment 0; a column that sees or shows nothing
+};
+template <bool KEYS>
+__device__ __forceinline__ ColumnRange column_range(const int *segments, int column0, int columns, int count, int lane) {
+  ColumnRange r = {0x7fffffff, -1, false, false};
+  bool shared = false, hidden = false;
+  for (int i = lane; i < count; i += kWave)
+    if (column0 + i < columns) {
+      const int v = segments != nullptr ? segments[column0 + i] : 0;
+      if (v < 0) hidden = true;
+      else if (KEYS && v == 0) shared = true;
+      else { r.lo = min(r.lo, v); r.hi = max(r.hi, v); }
+    }
+  for (int o = 32; o > 0; o >>= 1) {
+    r.lo = min(r.lo, __shfl_xor(r.lo, o, kWave));
+    r.hi = max(r.hi, __shfl_xor(r.hi, o, kWave));
   }
-  r.slope_factor = 0.f;
-  if (p.slopes != nullptr) {
-    const float *a = p.q_points + ((long long)b * p.nq + i) * 2, *c = p.k_points + ((long long)b * p.nk + j) * 2;
-    const float dx = a[0] - c[0], dy = a[1] - c[1];
-    r.slope_factor = sqrtf(fmaf(dx, dx, dy * dy));
-    r.s = fmaf(-p.slopes[head], r.slope_factor, r.s);
-  }
+  r.shared = __ballot(shared) != 0;
+  r.hidden = __ballot(hidden) != 0;
   return r;
 }
-__device__ __forceinline__ bool sees(const AttnLaunch &p, int b, int i, int j) {
-  if (p.k_segments == nullptr) return true;
-  const int mine = p.q_segments != nullptr ? p.q_segments[(long long)b * p.nq + i] : 0, theirs = p.k_segments[(long long)b * p.nk + j];
-  return mine >= 0 && (theirs == mine || theirs == 0);
+// By a row's number: whether some column sees it (shows itself to it), and whether all do.
+template <bool KEYS>
+__device__ __forceinline__ bool some_pair(const ColumnRange &c, int row) {
+  const bool within = row >= c.lo && row <= c.hi;
+  return KEYS ? row >= 0 && (c.shared || within) : c.hi >= 0 && (row == 0 || within);
+}
+template <bool KEYS>
+__device__ __forceinline__ bool every_pair(const ColumnRange &c, int row) {
+  if (c.hidden) return false;
+  return KEYS ? row >= 0 && (c.hi < 0 || (c.lo == row && c.hi == row)) : row == 0 || (c.lo == row && c.hi == row);
 }
 
-// A row of a tensor into a wave's LDS.
-template <typename Tag>
-__device__ __forceinline__ void park_row(float *dst, const char *row, int width, int lane) {
-  if (lane * 8 < width) {
-    float f[8];
-    load8<Tag>(row, lane * 8, f);
-#pragma unroll
-    for (int c = 0; c < 8; ++c) dst[lane * 8 + c] = f[c];
+struct TileMasks {
+  uint64_t some, every;      // bit t: tile t of up to 64
+};
+// Rows first .. last - 1; all waves together.  flags: 64 bytes of LDS, free again behind the next barrier.
+template <int RT, bool KEYS>
+__device__ __forceinline__ TileMasks tile_masks(const int *row_segments, bool masked, const ColumnRange &c, int first, int last, char *flags, int wave, int lane) {
+  const int tiles = min(64, (last - first + RT - 1) / RT);
+  if (!masked) {
+    TileMasks m;
+    m.some = tiles == 64 ? ~0ull : (1ull << tiles) - 1;
+    m.every = first + tiles * RT <= last ? m.some : m.some >> 1;
+    return m;
   }
-}
-// acc[u] += weight of lane l's row times its elements at lane and lane + 64, over all lanes; rows of weight 0 are not read.
-template <typename Tag, typename RowAt>
-__device__ __forceinline__ void add_rows(float (&acc)[2], float weight, int width, int lane, RowAt row_at) {
-  uint64_t left = __ballot(weight != 0.f);
-  while (left != 0) {
-    const int l = __builtin_ctzll(left);
-    left &= left - 1;
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), l));
-    const char *row = row_at(l);
+  for (int t = wave; t < tiles; t += kWaves) {
+    bool some = false, every = true;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int d = lane + u * 64;
-      if (d < width) {
-        float f[1];
-        Pack<Tag, 1>::decode(reinterpret_cast<const typename RawWord<Tag::kBytes>::type *>(row)[d], f);
-        acc[u] = fmaf(w, f[0], acc[u]);
+    for (int u = 0; u < RT / 64; ++u) {
+      const int row = first + t * RT + u * 64 + lane;
+      const int v = row < last ? (row_segments != nullptr ? row_segments[row] : 0) : kHiddenColumn;
+      some = some || some_pair<KEYS>(c, v);
+      every = every && row < last && every_pair<KEYS>(c, v);
+    }
+    const uint64_t has = __ballot(some), all = __ballot(every);
+    if (lane == 0) flags[t] = (char)((has != 0) | (all == ~0ull) << 1);
+  }
+  __syncthreads();
+  const int mine = lane < tiles ? flags[lane] : 0;
+  return {__ballot(mine & 1), __ballot(mine & 2)};
+}
+
+// What a thread carries of a row beside the tensors.
+struct RowLoads {
+  int segment;
+  f32x2 point;
+  float lse, delta;
+};
+
+// Walks the tiles: request(row0) starts the loads of a tile, put(tile, row0, every) brings what came into LDS, work(tile, every) computes.
+// A tile's loads are under way while the one before is worked on; two tiles of LDS in turn, one barrier a tile.
+template <typename S, bool KEYS, typename Request, typename Put, typename Work>
+__device__ __forceinline__ void walk_tiles(const int *row_segments, bool masked, const ColumnRange &c, int first, int last, char *lds, char *flags, int wave,
+                                           int lane, Request request, Put put, Work work) {
+  for (int window = first; window < last; window += 64 * S::RT) {
+    TileMasks m = tile_masks<S::RT, KEYS>(row_segments, masked, c, window, last, flags, wave, lane);
+    if (m.some != 0) {
+      auto take = [&](bool &every) {
+        const int t = __builtin_ctzll(m.some);
+        m.some &= m.some - 1;
+        every = m.every >> t & 1;
+        return window + t * S::RT;
+      };
+      bool every;
+      int row0 = take(every), turn = 0;
+      request(row0);
+      put(lds, row0, every);
+      __syncthreads();
+      for (;;) {
+        const bool more = m.some != 0;
+        bool next_every = false;
+        if (more) {
+          row0 = take(next_every);
+          request(row0);
+        }
+        work(lds + turn * S::kTileBytes, every);
+        if (!more) break;
+        turn ^= 1;
+        every = next_every;
+        put(lds + turn * S::kTileBytes, row0, every);
+        __syncthreads();
       }
     }
+    __syncthreads();
   }
 }
-template <typename Tag>
-__device__ __forceinline__ void write_row(void *base, long long row, const float (&acc)[2], float factor, int width, int lane) {
+
+// Where a workgroup stands: [batch][head][column tile][chunk], neighbours on one XCD.
+struct Place {
+  int b, head, tile, chunk;
+  __device__ __forceinline__ Place(int heads, int tiles, int chunks) {
+    int id = (int)xcd_contiguous_block(blockIdx.x, gridDim.x);
+    chunk = id % chunks; id /= chunks;
+    tile = id % tiles; id /= tiles;
+    head = id % heads;
+    b = id / heads;
+  }
+};
+
+// Sums of a column tile over the waves that divided the rows, through LDS: acc of wave (RW index) 0 .. RW - 1 times its factor.
+// Afterwards wave w holds the sums of the width blocks w, w + RW, ... and `mine` says so.
+template <typename S>
+__device__ __forceinline__ void merge_rows(f32x4 (&acc)[S::kWidthBlocks][S::CF], char *lds, int row_wave, int column_wave, int lane) {
+  if constexpr (S::RW > 1) {
+    constexpr int pitch = S::W + 4;
+    float *s = reinterpret_cast<float *>(lds);
+    const int g = lane >> 4, c = lane & 15;
+    __syncthreads();
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int d = lane + u * 64;
-    const float f[1] = {acc[u] * factor};
-    if (d < width) reinterpret_cast<typename RawWord<Tag::kBytes>::type *>(base)[row * width + d] = Pack<Tag, 1>::encode(f);
-  }
-}
-
-template <typename Tag>
-__global__ void __launch_bounds__(kRowThreads) attn_rows_forward_kernel(const AttnLaunch p) {
-  __shared__ float s_row[kRowWaves][kMaxAttnWidth];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const long long row = (long long)blockIdx.x * kRowWaves + wave;
-  if (row >= (long long)p.batch * p.nq * p.heads) return;
-  const int head = (int)(row % p.heads), i = (int)(row / p.heads % p.nq), b = (int)(row / p.heads / p.nq);
-  const int kv = head / (p.heads / p.kv_heads);
-  float *mine = s_row[wave];
-  park_row<Tag>(mine, row_of<Tag>(p.q, b, i, head), p.width, lane);
-  float top = -kInf, sum = 0.f, acc[2] = {0.f, 0.f};
-  for (int j0 = 0; j0 < p.nk; j0 += kWave) {
-    const int j = j0 + lane;
-    float s = -kInf;
-    if (j < p.nk && sees(p, b, i, j)) s = finish_score(p, dot_row<Tag>(row_of<Tag>(p.k, b, j, kv), mine, p.width), b, head, i, j).s;
-    const float now = fmaxf(top, wave_max(s));
-    if (now == -kInf) continue;
-    const float w = expf(s - now), keep = expf(top - now);
-    sum = fmaf(sum, keep, wave_sum(w));
-    acc[0] *= keep;
-    acc[1] *= keep;
-    top = now;
-    add_rows<Tag>(acc, w, p.width, lane, [&](int l) { return row_of<Tag>(p.v, b, j0 + l, kv); });
-  }
-  const bool empty = sum == 0.f;
-  write_row<Tag>(p.out, row, acc, empty ? 0.f : 1.f / sum, p.width, lane);
-  if (p.lse != nullptr && lane == 0) p.lse[((long long)b * p.heads + head) * p.nq + i] = empty ? kInf : top + logf(sum);
-}
-
-// grad_q, the rows' delta and their part of the slopes' gradient
-template <typename Tag>
-__global__ void __launch_bounds__(kRowThreads) attn_rows_grad_q_kernel(const AttnLaunch p, float *delta_out, float *slope_part) {
-  __shared__ float s_row[kRowWaves][2][kMaxAttnWidth];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const long long row = (long long)blockIdx.x * kRowWaves + wave;
-  if (row >= (long long)p.batch * p.nq * p.heads) return;
-  const int head = (int)(row % p.heads), i = (int)(row / p.heads % p.nq), b = (int)(row / p.heads / p.nq);
-  const int kv = head / (p.heads / p.kv_heads);
-  float *query = s_row[wave][0], *grad = s_row[wave][1];
-  park_row<Tag>(query, row_of<Tag>(p.q, b, i, head), p.width, lane);
-  park_row<Tag>(grad, row_of<Tag>(p.grad_out, b, i, head), p.width, lane);
-  const long long at = ((long long)b * p.heads + head) * p.nq + i;
-  const float delta = dot_row<Tag>(static_cast<const char *>(p.out) + row * p.width * Tag::kBytes, grad, p.width), lse = p.lse[at];
-  float acc[2] = {0.f, 0.f}, slope = 0.f;
-  for (int j0 = 0; j0 < p.nk; j0 += kWave) {
-    const int j = j0 + lane;
-    float dx = 0.f;
-    if (j < p.nk && sees(p, b, i, j)) {
-      const Score s = finish_score(p, dot_row<Tag>(row_of<Tag>(p.k, b, j, kv), query, p.width), b, head, i, j);
-      const float ds = expf(s.s - lse) * (dot_row<Tag>(row_of<Tag>(p.v, b, j, kv), grad, p.width) - delta);
-      slope = fmaf(-ds, s.slope_factor, slope);
-      dx = ds * s.bent;
-    }
-    add_rows<Tag>(acc, dx, p.width, lane, [&](int l) { return row_of<Tag>(p.k, b, j0 + l, kv); });
-  }
-  if (p.grad_q != nullptr) write_row<Tag>(p.grad_q, row, acc, p.scale, p.width, lane);
-  slope = wave_sum(slope);
-  if (lane == 0) {
-    delta_out[at] = delta;
-    if (slope_part != nullptr) slope_part[at] = slope;
-  }
-}
-
-template <typename Tag>
-__global__ void __launch_bounds__(kRowThreads) attn_rows_grad_kv_kernel(const AttnLaunch p, const float *delta) {
-  __shared__ float s_row[kRowWaves][2][kMaxAttnWidth];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const long long row = (long long)blockIdx.x * kRowWaves + wave;
-  if (row >= (long long)p.batch * p.nk * p.kv_heads) return;
-  const int kv = (int)(row % p.kv_heads), j = (int)(row / p.kv_heads % p.nk), b = (int)(row / p.kv_heads / p.nk);
-  const int share = p.heads / p.kv_heads;
-  float *key = s_row[wave][0], *value = s_row[wave][1];
-  park_row<Tag>(key, row_of<Tag>(p.k, b, j, kv), p.width, lane);
-  park_row<Tag>(value, row_of<Tag>(p.v, b, j, kv), p.width, lane);
-  float dk[2] = {0.f, 0.f}, dv[2] = {0.f, 0.f};
-  for (int head = kv * share; head < (kv + 1) * share; ++head)
-    for (int i0 = 0; i0 < p.nq; i0 += kWave) {
-      const int i = i0 + lane;
-      float weight = 0.f, dx = 0.f;
-      if (i < p.nq && sees(p, b, i, j)) {
-        const long long at = ((long long)b * p.heads + head) * p.nq + i;
-        const Score s = finish_score(p, dot_row<Tag>(row_of<Tag>(p.q, b, i, head), key, p.width), b, head, i, j);
-        weight = expf(s.s - p.lse[at]);
-        dx = weight * (dot_row<Tag>(row_of<Tag>(p.grad_out, b, i, head), value, p.width) - delta[at]) * s.bent;
+    for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+      for (int d = 0; d < S::kWidthBlocks; ++d)
+        *reinterpret_cast<f32x4 *>(s + (size_t)(((row_wave * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c) * pitch + d * 16 + g * 4) = acc[d][f];
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+      for (int d = 0; d < S::kWidthBlocks; ++d) {
+        if (d % S::RW != row_wave) continue;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < S::RW; ++w)
+          sum += *reinterpret_cast<const f32x4 *>(s + (size_t)(((w * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c) * pitch + d * 16 + g * 4);
+        acc[d][f] = sum;
       }
-      add_rows<Tag>(dv, weight, p.width, lane, [&](int l) { return row_of<Tag>(p.grad_out, b, i0 + l, head); });
-      add_rows<Tag>(dk, dx, p.width, lane, [&](int l) { return row_of<Tag>(p.q, b, i0 + l, head); });
+  }
+}
+template <typename S>
+__device__ __forceinline__ bool holds(int width_block, int row_wave) { return S::RW == 1 || width_block % S::RW == row_wave; }
+
+template <typename Tag>
+__device__ __forceinline__ void store4(void *base, size_t element, f32x4 v) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  reinterpret_cast<typename RawWord<4 * Tag::kBytes>::type *>(base)[element / 4] = Pack<Tag, 4>::encode(f);
+}
+// What rounding took from v, in the type.
+template <typename Tag>
+__device__ __forceinline__ f32x4 rounded_off(f32x4 v) {
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  float r[4];
+  Pack<Tag, 4>::decode(Pack<Tag, 4>::encode(f), r);
+  return f32x4{f[0] - r[0], f[1] - r[1], f[2] - r[2], f[3] - r[3]};
+}
+
+// ---------------------------------------------------------------- forward
+struct Split {
+  int tiles, chunks, chunk_rows;      // column tiles of a head; parts of the rows, a whole number of tiles each
+  float *part, *stats;                // [chunk][batch][query][head][width], [..][2]: unnormalised sums, maximum and sum
+};
+
+template <typename S>
+__global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch p, const Split split) {
+  typedef typename S::Tag Tag;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ char s_flags[64];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
+  const int row_wave = wave / S::kColumnWaves, column_wave = wave % S::kColumnWaves;
+  const Place at(p.heads, split.tiles, split.chunks);
+  const int kv = at.head / (p.heads / p.kv_heads), width_bytes = p.width * Tag::kBytes;
+  const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
+  const int first = at.chunk * split.chunk_rows, last = min(p.nk, first + split.chunk_rows);
+  const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
+  const Scores scores(p, at.head);
+  const bool plain = scores.as_they_are(), masked = p.k_segments != nullptr;
+  const float factor = plain ? scores.factor : 1.f;
+
+  u32x4 q[S::CF][S::kSlices];
+  load_columns<S>(q, head_rows<Tag>(p.q, at.b, at.head), mine0, p.nq, width_bytes, lane);
+  const int *q_segments = p.q_segments != nullptr ? p.q_segments + (long long)at.b * p.nq : nullptr;
+  const int *k_segments = masked ? p.k_segments + (long long)at.b * p.nk : nullptr;
+  int segment[S::CF];
+  f32x2 point[S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const int i = mine0 + 16 * f + c;
+    segment[f] = i < p.nq ? (q_segments != nullptr ? q_segments[i] : 0) : kHiddenColumn;
+    if (segment[f] < 0) segment[f] = kHiddenColumn;
+    point[f] = f32x2{0.f, 0.f};
+    if (scores.apart && i < p.nq) point[f] = reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + i];
+  }
+  const ColumnRange range = masked ? column_range<false>(q_segments, column0, p.nq, S::kColumns, lane) : ColumnRange{};
+
+  f32x4 acc[S::kWidthBlocks][S::CF], total[S::CF];
+  float top[S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    top[f] = -kInf;
+    total[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  TileLoads<S> next_k, next_v;
+  RowLoads next = {};
+  auto request = [&](int row0) {
+    next_k.request(keys, row0, last, width_bytes, wave, lane);
+    next_v.request(values, row0, last, width_bytes, wave, lane);
+    const int row = row0 + (int)threadIdx.x;
+    if ((int)threadIdx.x < S::RT) {
+      next.segment = row < last ? (masked ? k_segments[row] : 0) : -1;
+      if (scores.apart) next.point = row < last ? reinterpret_cast<const f32x2 *>(p.k_points)[(long long)at.b * p.nk + row] : f32x2{0.f, 0.f};
     }
-  if (p.grad_k != nullptr) write_row<Tag>(p.grad_k, row, dk, p.scale, p.width, lane);
-  if (p.grad_v != nullptr) write_row<Tag>(p.grad_v, row, dv, 1.f, p.width, lane);
+  };
+  auto put = [&](char *tile, int, bool every) {
+    if (!every)
+#pragma unroll
+      for (int u = 0; u < S::RT / 64; ++u) put_poison<S>(tile, u, next_v.clear_bad(u), wave, lane);
+    next_k.put(tile, wave, lane);
+    next_v.put(tile + S::kTensorBytes, wave, lane);
+    if ((int)threadIdx.x < S::RT) {
+      reinterpret_cast<int *>(tile + S::kSegments)[threadIdx.x] = next.segment;
+      if (scores.apart) reinterpret_cast<f32x2 *>(tile + S::kPoints)[threadIdx.x] = next.point;
+    }
+  };
+  auto work = [&](const char *tile, bool every) {
+    const int block0 = row_wave * S::kRowBlocks;
+    f32x4 s[S::kRowBlocks][S::CF];
+#pragma unroll
+    for (int n = 0; n < S::kRowBlocks; ++n) {
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) s[n][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int sl = 0; sl < S::kSlices; ++sl) {
+        const u32x4 a = fragment<S>(tile, block0 + n, sl, lane);
+#pragma unroll
+        for (int f = 0; f < S::CF; ++f) s[n][f] = mfma_64_bytes<Tag>(a, q[f][sl], s[n][f]);
+      }
+    }
+    if (!plain)
+#pragma unroll
+      for (int n = 0; n < S::kRowBlocks; ++n) {
+        const f32x2 *from = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + (block0 + n) * 16 + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f32x2 other = {0.f, 0.f};
+          if (scores.apart) other = from[r];
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) {
+            float v = (scores.bent ? scores.tanh_of<Tag>(s[n][f][r]) : s[n][f][r]) * scores.factor;
+            if (scores.apart) v = fmaf(-scores.slope, distance(point[f], other), v);
+            s[n][f][r] = v;
+          }
+        }
+      }
+    if (!every)
+#pragma unroll
+      for (int n = 0; n < S::kRowBlocks; ++n) {
+        const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + (block0 + n) * 16 + 4 * g;
+        const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + (block0 + n) * 16 + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) s[n][f][r] = segments[r] == 0 || segments[r] == segment[f] ? s[n][f][r] + poison[r] : -kInf;
+      }
+    // the maximum moves where a score passes it by 2^8
+    float high[S::CF];
+    bool passed = false;
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      high[f] = fmaxf(fmaxf(s[0][f][0], s[0][f][1]), fmaxf(s[0][f][2], s[0][f][3]));
+#pragma unroll
+      for (int n = 1; n < S::kRowBlocks; ++n) high[f] = max3(max3(high[f], s[n][f][0], s[n][f][1]), s[n][f][2], s[n][f][3]);
+      passed = passed || high[f] * factor > top[f] + 8.f;
+    }
+    if (__ballot(passed) != 0)
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) {
+        const float now = fmaxf(top[f], column_max(high[f]) * factor);
+        const float keep = __builtin_amdgcn_exp2f(top[f] - (now == -kInf ? 0.f : now));
+        top[f] = now;
+#pragma unroll
+        for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] *= keep;
+        total[f] *= keep;
+      }
+#pragma unroll
+    for (int n = 0; n < S::kRowBlocks; n += 2) {
+      f32x4 w[2][S::CF];
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) {
+        const float off = kForwardShift<Tag> - (top[f] == -kInf ? 0.f : top[f]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[n + h][f][r], factor, off));
+          if constexpr (Tag::kBytes == 4) total[f] += w[h][f];
+        }
+        if constexpr (Tag::kBytes == 2) {      // of the weights as the product takes them
+          constexpr uint32_t one = Tag::kCode == F16::kCode ? 0x3c003c00u : 0x3f803f80u;
+          const float v[8] = {w[0][f].x, w[0][f].y, w[0][f].z, w[0][f].w, w[1][f].x, w[1][f].y, w[1][f].z, w[1][f].w};
+          total[f] = mfma_64_bytes<Tag>(u32x4{one, one, one, one}, Pack<Tag, 8>::encode(v), total[f]);
+        }
+      }
+      add_product<S>(acc, tile + S::kTensorBytes, block0 + n, w, lane);
+    }
+  };
+  walk_tiles<S, false>(k_segments, masked, range, first, last, lds, s_flags, wave, lane, request, put, work);
+
+  float sum[S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    sum[f] = Tag::kBytes == 4 ? column_sum((total[f].x + total[f].y) + (total[f].z + total[f].w)) : total[f].x;
+    if (segment[f] < 0) {      // sees nothing
+      sum[f] = 0.f;
+      top[f] = -kInf;
+#pragma unroll
+      for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  if constexpr (S::RW > 1) {
+    f32x2 *s_stats = reinterpret_cast<f32x2 *>(lds + kWaves * 16 * S::CF * (S::W + 4) * 4);
+    auto slot = [&](int w, int f) { return ((w * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c; };
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f)
+      if (g == 0) s_stats[slot(row_wave, f)] = f32x2{top[f], sum[f]};
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      const float was = top[f];
+      float now = -kInf;
+#pragma unroll
+      for (int w = 0; w < S::RW; ++w) now = fmaxf(now, s_stats[slot(w, f)].x);
+      const float base = now == -kInf ? 0.f : now;
+      sum[f] = 0.f;
+#pragma unroll
+      for (int w = 0; w < S::RW; ++w) sum[f] = fmaf(s_stats[slot(w, f)].y, __builtin_amdgcn_exp2f(s_stats[slot(w, f)].x - base), sum[f]);
+      const float keep = __builtin_amdgcn_exp2f(was - base);
+      top[f] = now;
+#pragma unroll
+      for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] *= keep;
+    }
+    merge_rows<S>(acc, lds, row_wave, column_wave, lane);
+  }
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const int i = mine0 + 16 * f + c;
+    if (i >= p.nq) continue;
+    const size_t row = ((size_t)at.b * p.nq + i) * p.heads + at.head;
+    const bool split_rows = split.chunks > 1;
+    const size_t part_row = ((size_t)at.chunk * p.batch * p.nq * p.heads + row);
+    const float inv = sum[f] == 0.f ? 0.f : 1.f / sum[f];
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) {
+      const int column = d * 16 + g * 4;
+      if (!holds<S>(d, row_wave) || column >= p.width) continue;
+      if (split_rows) {
+        *reinterpret_cast<f32x4 *>(split.part + part_row * p.width + column) = acc[d][f];
+      } else {
+        const f32x4 v = acc[d][f] * inv;
+        store4<Tag>(p.out, row * p.width + column, v);
+        if (p.out_rest != nullptr) store4<Tag>(p.out_rest, row * p.width + column, rounded_off<Tag>(v));
+      }
+    }
+    if (g != 0 || row_wave != 0) continue;
+    if (split_rows) reinterpret_cast<f32x2 *>(split.stats)[part_row] = f32x2{top[f], sum[f]};
+    else if (p.lse != nullptr)
+      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = sum[f] == 0.f ? kInf : top[f] - kForwardShift<Tag> + __builtin_amdgcn_logf(sum[f]);
+  }
+}
+
+// The chunks of a row: a lane takes four elements.
+template <typename Tag>
+__global__ void __launch_bounds__(kThreads) attn_join_kernel(const AttnLaunch p, const Split split) {
+  const int lanes = p.width / 4;
+  const long long rows = (long long)p.batch * p.nq * p.heads, id = (long long)blockIdx.x * kThreads + threadIdx.x;
+  const long long row = id / lanes;
+  const int column = (int)(id % lanes) * 4;
+  if (row >= rows) return;
+  const f32x2 *stats = reinterpret_cast<const f32x2 *>(split.stats);
+  float top = -kInf;
+  for (int k = 0; k < split.chunks; ++k) top = fmaxf(top, stats[k * rows + row].x);
+  const float base = top == -kInf ? 0.f : top;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < split.chunks; ++k) {
+    const f32x2 s = stats[k * rows + row];
+    const float w = __builtin_amdgcn_exp2f(s.x - base);
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(split.part + (k * rows + row) * p.width + column);
+    sum = fmaf(w, s.y, sum);
+    acc += v * w;
+  }
+  acc *= sum == 0.f ? 0.f : 1.f / sum;
+  store4<Tag>(p.out, row * p.width + column, acc);
+  if (p.out_rest != nullptr) store4<Tag>(p.out_rest, row * p.width + column, rounded_off<Tag>(acc));
+  if (p.lse != nullptr && column == 0) {
+    const long long head = row % p.heads, i = row / p.heads % p.nq, b = row / p.heads / p.nq;
+    p.lse[(b * p.heads + head) * p.nq + i] = sum == 0.f ? kInf : top - kForwardShift<Tag> + __builtin_amdgcn_logf(sum);
+  }
+}
+
+// ---------------------------------------------------------------- backward
+// dX in fp16: a column's values are kept in the type's normal range by a power of two of its own, chosen when one first leaves it
+// (the largest goes to 2^13), and the sums follow.  Gradients of loss-scaled or averaged losses and weights of thousands of keys
+// would round to subnormals otherwise.
+template <typename S>
+struct ColumnScale {
+  static constexpr bool kNeeded = S::Tag::kCode == F16::kCode;
+  float by[S::CF];
+  __device__ __forceinline__ ColumnScale() {
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) by[f] = kNeeded ? 0x1p100f : 1.f;
+  }
+  __device__ __forceinline__ void apply(f32x4 (&v)[2][S::CF], f32x4 (&acc)[S::kWidthBlocks][S::CF]) {
+    if constexpr (kNeeded) {
+      float high[S::CF];
+      bool passed = false;
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) {
+        high[f] = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) high[f] = max3(max3(high[f], fabsf(v[h][f].x), fabsf(v[h][f].y)), fabsf(v[h][f].z), fabsf(v[h][f].w));
+        passed = passed || high[f] * by[f] > 32768.f;
+      }
+      if (__ballot(passed) != 0)
+#pragma unroll
+        for (int f = 0; f < S::CF; ++f) {
+          const float most = column_max(high[f]);
+          if (most * by[f] > 32768.f) {
+            const int e = 267 - (int)(__builtin_bit_cast(uint32_t, most) >> 23);
+            const float now = __builtin_bit_cast(float, (uint32_t)max(1, min(e, 227)) << 23);
+            const float ratio = now / by[f];
+            by[f] = now;
+#pragma unroll
+            for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] *= ratio;
+          }
+        }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int f = 0; f < S::CF; ++f) v[h][f] *= by[f];
+    }
+  }
+};
+
+// Scores of 32 rows, from the products: rows' positions in `other`.  far, bend: the distances and 1 - tanh^2, for the gradients.
+template <typename S, typename Points>
+__device__ __forceinline__ void finish_scores(const Scores &scores, f32x4 (&s)[2][S::CF], f32x4 (&far)[2][S::CF], f32x4 (&bend)[2][S::CF],
+                                              const f32x2 (&point)[S::CF], Points other) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f32x2 there = {0.f, 0.f};
+      if (scores.apart) there = other(h, r);
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) {
+        float v = s[h][f][r];
+        if (scores.bent) {
+          v = scores.tanh_of<typename S::Tag>(v);
+          bend[h][f][r] = fmaf(-v, v, 1.f);
+        }
+        v *= scores.factor;
+        if (scores.apart) {
+          far[h][f][r] = distance(point[f], there);
+          v = fmaf(-scores.slope, far[h][f][r], v);
+        }
+        s[h][f][r] = v;
+      }
+    }
+}
+
+struct BackwardParts {
+  float *delta, *slopes;      // (batch, heads, queries); (batch, heads, column tiles)
+  int tiles;
+};
+
+// dQ, delta and the slopes' parts: columns are queries, rows keys.
+template <typename S>
+__global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnLaunch p, const BackwardParts parts) {
+  typedef typename S::Tag Tag;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ char s_flags[64];
+  __shared__ float s_slopes[kWaves];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
+  const int row_wave = wave / S::kColumnWaves, column_wave = wave % S::kColumnWaves;
+  const Place at(p.heads, parts.tiles, 1);
+  const int kv = at.head / (p.heads / p.kv_heads), width_bytes = p.width * Tag::kBytes;
+  const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
+  const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
+  const Scores scores(p, at.head);
+  const bool plain = scores.as_they_are(), masked = p.k_segments != nullptr;
+  const float factor = plain ? scores.factor : 1.f;
+
+  u32x4 q[S::CF][S::kSlices], go[S::CF][S::kSlices];
+  load_columns<S>(q, head_rows<Tag>(p.q, at.b, at.head), mine0, p.nq, width_bytes, lane);
+  load_columns<S>(go, head_rows<Tag>(p.grad_out, at.b, at.head), mine0, p.nq, width_bytes, lane);
+  float delta[S::CF];
+  {
+    const long long token = (long long)p.heads * p.width;
+    u32x4 o[S::CF][S::kSlices];
+    load_columns<S>(o, head_rows<Tag>(AttnRows{p.out, token * p.nq, token, p.width}, at.b, at.head), mine0, p.nq, width_bytes, lane);
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      delta[f] = 0.f;
+#pragma unroll
+      for (int s = 0; s < S::kSlices; ++s) delta[f] = dot_16_bytes<Tag>(go[f][s], o[f][s], delta[f]);
+    }
+    if (p.out_rest != nullptr) {
+      load_columns<S>(o, head_rows<Tag>(AttnRows{p.out_rest, token * p.nq, token, p.width}, at.b, at.head), mine0, p.nq, width_bytes, lane);
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+        for (int s = 0; s < S::kSlices; ++s) delta[f] = dot_16_bytes<Tag>(go[f][s], o[f][s], delta[f]);
+    }
+  }
+  const int *q_segments = p.q_segments != nullptr ? p.q_segments + (long long)at.b * p.nq : nullptr;
+  const int *k_segments = masked ? p.k_segments + (long long)at.b * p.nk : nullptr;
+  int segment[S::CF];
+  f32x2 point[S::CF];
+  float lse[S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const int i = mine0 + 16 * f + c;
+    const long long stat = ((long long)at.b * p.heads + at.head) * p.nq + i;
+    segment[f] = i < p.nq ? (q_segments != nullptr ? q_segments[i] : 0) : kHiddenColumn;
+    if (segment[f] < 0) segment[f] = kHiddenColumn;
+    point[f] = f32x2{0.f, 0.f};
+    if (scores.apart && i < p.nq) point[f] = reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + i];
+    lse[f] = i < p.nq ? p.lse[stat] : kInf;
+    delta[f] = column_sum(delta[f]);
+    if (i < p.nq && g == 0 && row_wave == 0) parts.delta[stat] = delta[f];
+  }
+  const ColumnRange range = masked ? column_range<false>(q_segments, column0, p.nq, S::kColumns, lane) : ColumnRange{};
+
+  f32x4 acc[S::kWidthBlocks][S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  ColumnScale<S> up;
+  float slope[S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) slope[f] = 0.f;
+
+  TileLoads<S> next_k, next_v;
+  RowLoads next = {};
+  auto request = [&](int row0) {
+    next_k.request(keys, row0, p.nk, width_bytes, wave, lane);
+    next_v.request(values, row0, p.nk, width_bytes, wave, lane);
+    const int row = row0 + (int)threadIdx.x;
+    if ((int)threadIdx.x < S::RT) {
+      next.segment = row < p.nk ? (masked ? k_segments[row] : 0) : -1;
+      if (scores.apart) next.point = row < p.nk ? reinterpret_cast<const f32x2 *>(p.k_points)[(long long)at.b * p.nk + row] : f32x2{0.f, 0.f};
+    }
+  };
+  auto put = [&](char *tile, int, bool every) {
+    if (!every)
+#pragma unroll
+      for (int u = 0; u < S::RT / 64; ++u) put_poison<S>(tile, u, next_k.clear_bad(u), wave, lane);
+    next_k.put(tile, wave, lane);
+    next_v.put(tile + S::kTensorBytes, wave, lane);
+    if ((int)threadIdx.x < S::RT) {
+      reinterpret_cast<int *>(tile + S::kSegments)[threadIdx.x] = next.segment;
+      if (scores.apart) reinterpret_cast<f32x2 *>(tile + S::kPoints)[threadIdx.x] = next.point;
+    }
+  };
+  auto work = [&](const char *tile, bool every) {
+#pragma unroll
+    for (int n = 0; n < S::kRowBlocks; n += 2) {
+      const int block = row_wave * S::kRowBlocks + n;
+      f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int f = 0; f < S::CF; ++f) s[h][f] = t[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int sl = 0; sl < S::kSlices; ++sl) {
+          const u32x4 a = fragment<S>(tile, block + h, sl, lane), b = fragment<S>(tile + S::kTensorBytes, block + h, sl, lane);
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) {
+            s[h][f] = mfma_64_bytes<Tag>(a, q[f][sl], s[h][f]);
+            t[h][f] = mfma_64_bytes<Tag>(b, go[f][sl], t[h][f]);
+          }
+        }
+      }
+      const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
+      if (!plain) finish_scores<S>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
+      const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
+      const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) {
+            float x = s[h][f][r];
+            if (!every) x += poison[h * 16 + r];
+            float ds = __builtin_amdgcn_exp2f(fmaf(x, factor, -lse[f])) * (t[h][f][r] - delta[f]);
+            if (!every) ds = segments[h * 16 + r] == 0 || segments[h * 16 + r] == segment[f] ? ds : 0.f;
+            s[h][f][r] = ds;
+          }
+      if (scores.apart)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int f = 0; f < S::CF; ++f) {
+              // a distance to a place that is not seen may be anything
+              const float apart = every || s[h][f][r] != 0.f ? far[h][f][r] : 0.f;
+              slope[f] = fmaf(-s[h][f][r], apart, slope[f]);
+            }
+      if (scores.bent)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[h][f][r] = every || s[h][f][r] != 0.f ? s[h][f][r] * bend[h][f][r] : 0.f;
+      up.apply(s, acc);
+      add_product<S>(acc, tile, block, s, lane);
+    }
+  };
+  walk_tiles<S, false>(k_segments, masked, range, 0, p.nk, lds, s_flags, wave, lane, request, put, work);
+
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const float by = p.scale / up.by[f];
+    const bool sees = segment[f] >= 0;
+    if (!sees) slope[f] = 0.f;
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = sees ? acc[d][f] * by : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  merge_rows<S>(acc, lds, row_wave, column_wave, lane);
+  if (p.grad_q != nullptr)
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      const int i = mine0 + 16 * f + c;
+      if (i >= p.nq) continue;
+      const size_t row = ((size_t)at.b * p.nq + i) * p.heads + at.head;
+#pragma unroll
+      for (int d = 0; d < S::kWidthBlocks; ++d)
+        if (holds<S>(d, row_wave) && d * 16 + g * 4 < p.width) store4<Tag>(p.grad_q, row * p.width + d * 16 + g * 4, acc[d][f]);
+    }
+  if (parts.slopes != nullptr) {
+    float sum = 0.f;
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) sum += slope[f];
+    sum = cluster_sum(sum, kWave);
+    if (lane == 0) s_slopes[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) parts.slopes[((size_t)at.b * p.heads + at.head) * parts.tiles + at.tile] = (s_slopes[0] + s_slopes[1]) + (s_slopes[2] + s_slopes[3]);
+  }
+}
+
+// dK and dV: columns are keys, rows the queries of every head that shares the key head.
+template <typename S>
+__global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch p, const BackwardParts parts) {
+  typedef typename S::Tag Tag;
+  extern __shared__ __align__(16) char lds[];
+  __shared__ char s_flags[64];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
+  const int row_wave = wave / S::kColumnWaves, column_wave = wave % S::kColumnWaves;
+  const Place at(p.kv_heads, parts.tiles, 1);
+  const int share = p.heads / p.kv_heads, width_bytes = p.width * Tag::kBytes;
+  const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
+  const bool masked = p.k_segments != nullptr;
+
+  u32x4 k[S::CF][S::kSlices], v[S::CF][S::kSlices];
+  load_columns<S>(k, head_rows<Tag>(p.k, at.b, at.head), mine0, p.nk, width_bytes, lane);
+  load_columns<S>(v, head_rows<Tag>(p.v, at.b, at.head), mine0, p.nk, width_bytes, lane);
+  const int *q_segments = p.q_segments != nullptr ? p.q_segments + (long long)at.b * p.nq : nullptr;
+  const int *k_segments = masked ? p.k_segments + (long long)at.b * p.nk : nullptr;
+  // queries low .. low + span see a key: its own segment's, or all that are not negative
+  int low[S::CF];
+  uint32_t span[S::CF];
+  f32x2 point[S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const int j = mine0 + 16 * f + c, segment = j < p.nk ? (masked ? k_segments[j] : 0) : -1;
+    low[f] = max(segment, -1);
+    span[f] = segment == 0 ? 0x7fffffffu : 0u;
+    point[f] = f32x2{0.f, 0.f};
+    if (p.slopes != nullptr && j < p.nk) point[f] = reinterpret_cast<const f32x2 *>(p.k_points)[(long long)at.b * p.nk + j];
+  }
+  const ColumnRange range = masked ? column_range<true>(k_segments, column0, p.nk, S::kColumns, lane) : ColumnRange{};
+
+  f32x4 dk[S::kWidthBlocks][S::CF], dv[S::kWidthBlocks][S::CF];
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) dk[d][f] = dv[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  ColumnScale<S> up;
+
+  for (int head = at.head * share; head < (at.head + 1) * share; ++head) {
+    const HeadRows queries = head_rows<Tag>(p.q, at.b, head), grads = head_rows<Tag>(p.grad_out, at.b, head);
+    const Scores scores(p, head);
+    const bool plain = scores.as_they_are();
+    const float factor = plain ? scores.factor : 1.f;
+    TileLoads<S> next_q, next_g;
+    RowLoads next = {};
+    auto request = [&](int row0) {
+      next_q.request(queries, row0, p.nq, width_bytes, wave, lane);
+      next_g.request(grads, row0, p.nq, width_bytes, wave, lane);
+      const int row = row0 + (int)threadIdx.x;
+      if ((int)threadIdx.x < S::RT) {
+        const bool there = row < p.nq;
+        const long long stat = ((long long)at.b * p.heads + head) * p.nq + row;
+        next.segment = there ? (q_segments != nullptr ? q_segments[row] : 0) : kHiddenColumn;
+        next.lse = there ? p.lse[stat] : kInf;
+        next.delta = there ? parts.delta[stat] : 0.f;
+        if (scores.apart) next.point = there ? reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + row] : f32x2{0.f, 0.f};
+      }
+    };
+    auto put = [&](char *tile, int, bool every) {
+      if (!every)
+#pragma unroll
+        for (int u = 0; u < S::RT / 64; ++u) {
+          const bool bad_q = next_q.clear_bad(u), bad_g = next_g.clear_bad(u);
+          put_poison<S>(tile, u, bad_q || bad_g, wave, lane);
+        }
+      next_q.put(tile, wave, lane);
+      next_g.put(tile + S::kTensorBytes, wave, lane);
+      if ((int)threadIdx.x < S::RT) {
+        reinterpret_cast<int *>(tile + S::kSegments)[threadIdx.x] = max(next.segment, kHiddenColumn) == -1 ? kHiddenColumn : max(next.segment, kHiddenColumn);
+        reinterpret_cast<float *>(tile + S::kLse)[threadIdx.x] = next.lse - kBackwardShift<Tag>;
+        reinterpret_cast<float *>(tile + S::kDelta)[threadIdx.x] = next.delta;
+        if (scores.apart) reinterpret_cast<f32x2 *>(tile + S::kPoints)[threadIdx.x] = next.point;
+      }
+    };
+    auto work = [&](const char *tile, bool every) {
+#pragma unroll
+      for (int n = 0; n < S::kRowBlocks; n += 2) {
+        const int block = row_wave * S::kRowBlocks + n;
+        f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) s[h][f] = t[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int sl = 0; sl < S::kSlices; ++sl) {
+            const u32x4 a = fragment<S>(tile, block + h, sl, lane), b = fragment<S>(tile + S::kTensorBytes, block + h, sl, lane);
+#pragma unroll
+            for (int f = 0; f < S::CF; ++f) {
+              s[h][f] = mfma_64_bytes<Tag>(a, k[f][sl], s[h][f]);
+              t[h][f] = mfma_64_bytes<Tag>(b, v[f][sl], t[h][f]);
+            }
+          }
+        }
+        const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
+        if (!plain) finish_scores<S>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
+        const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
+        const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
+        const float *lse = reinterpret_cast<const float *>(tile + S::kLse) + block * 16 + 4 * g;
+        const float *delta = reinterpret_cast<const float *>(tile + S::kDelta) + block * 16 + 4 * g;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int f = 0; f < S::CF; ++f) {
+              float x = s[h][f][r];
+              if (!every) x += poison[h * 16 + r];
+              float w = __builtin_amdgcn_exp2f(fmaf(x, factor, -lse[h * 16 + r]));
+              float dx = w * (t[h][f][r] - delta[h * 16 + r]);
+              if (scores.bent) dx *= bend[h][f][r];
+              if (!every) {
+                const bool seen = (uint32_t)(segments[h * 16 + r] - low[f]) <= span[f];
+                w = seen ? w : 0.f;
+                dx = seen ? dx : 0.f;
+              }
+              s[h][f][r] = w;
+              t[h][f][r] = dx;
+            }
+        add_product<S>(dv, tile + S::kTensorBytes, block, s, lane);
+        up.apply(t, dk);
+        add_product<S>(dk, tile, block, t, lane);
+      }
+    };
+    walk_tiles<S, true>(q_segments, masked, range, 0, p.nq, lds, s_flags, wave, lane, request, put, work);
+  }
+
+  const float down = __builtin_amdgcn_exp2f(-kBackwardShift<Tag>);
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) {
+      dk[d][f] *= p.scale * down / up.by[f];
+      dv[d][f] *= down;
+    }
+  merge_rows<S>(dk, lds, row_wave, column_wave, lane);
+  merge_rows<S>(dv, lds, row_wave, column_wave, lane);
+#pragma unroll
+  for (int f = 0; f < S::CF; ++f) {
+    const int j = mine0 + 16 * f + c;
+    if (j >= p.nk) continue;
+    const size_t row = ((size_t)at.b * p.nk + j) * p.kv_heads + at.head;
+#pragma unroll
+    for (int d = 0; d < S::kWidthBlocks; ++d) {
+      if (!holds<S>(d, row_wave) || d * 16 + g * 4 >= p.width) continue;
+      if (p.grad_k != nullptr) store4<Tag>(p.grad_k, row * p.width + d * 16 + g * 4, dk[d][f]);
+      if (p.grad_v != nullptr) store4<Tag>(p.grad_v, row * p.width + d * 16 + g * 4, dv[d][f]);
+    }
+  }
 }
 
 // Sums of the slopes' parts of a head, [batch][heads][parts], in a fixed order.
-__global__ void __launch_bounds__(kRowThreads) attn_slope_grad_kernel(const float *part, float *grad, int batch, int heads, int parts) {
-  __shared__ float s_sum[kRowWaves];
+__global__ void __launch_bounds__(kThreads) attn_slope_grad_kernel(const float *part, float *grad, int batch, int heads, int parts) {
+  __shared__ float s_sum[kWaves];
   const int head = blockIdx.x, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   float sum = 0.f;
   for (int b = 0; b < batch; ++b)
-    for (int i = threadIdx.x; i < parts; i += kRowThreads) sum += part[((long long)b * heads + head) * parts + i];
-  sum = wave_sum(sum);
+    for (int i = threadIdx.x; i < parts; i += kThreads) sum += part[((size_t)b * heads + head) * parts + i];
+  sum = cluster_sum(sum, kWave);
   if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) grad[head] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
 }
 
-unsigned row_blocks(long long rows) { return (unsigned)((rows + kRowWaves - 1) / kRowWaves); }
-size_t rows_bytes(const AttnLaunch &p) { return ((size_t)p.batch * p.heads * p.nq * sizeof(float) + 255) / 256 * 256; }
+// ---------------------------------------------------------------- host
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-template <typename Tag>
-hipError_t forward_t(const AttnLaunch &p, hipStream_t stream) {
-  hipLaunchKernelGGL((attn_rows_forward_kernel<Tag>), dim3(row_blocks((long long)p.batch * p.nq * p.heads)), dim3(kRowThreads), 0, stream, p);
+enum Mode { kWide2, kWide1, kSplitRows };
+// Columns a workgroup: 128, 64, or 16 with the four waves dividing the rows.
+Mode column_mode(long long heads, int columns) {
+  if (heads * ceil_div(columns, 128) >= 512) return kWide2;
+  return heads * ceil_div(columns, 64) >= 256 ? kWide1 : kSplitRows;
+}
+template <typename Tag, int W>
+struct Modes {
+  static constexpr bool kLarge = W * Tag::kBytes > 256;
+  typedef Shape<Tag, W, 64, 1, kLarge ? 1 : 2> Wide2;
+  typedef Shape<Tag, W, 64, 1, 1> Wide1;
+  typedef Shape<Tag, W, kLarge ? 64 : 128, kLarge ? 2 : 4, 1> SplitRows;
+};
+
+template <typename S, typename... A>
+hipError_t run(void (*kernel)(A...), long long blocks, hipStream_t stream, A... args) {
+  if (S::kLdsBytes > (int)kMaxDynamicLds)
+    if (hipError_t e = ensure_dynamic_lds_limit(reinterpret_cast<const void *>(kernel), S::kLdsBytes)) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), S::kLdsBytes, stream, args...);
   return hipGetLastError();
 }
 
+// Few columns: the rows of a head are divided among workgroups too, a few tiles each, and joined behind.
+template <typename S>
+Split plan_forward(const AttnLaunch &p) {
+  Split s = {};
+  s.tiles = ceil_div(p.nq, S::kColumns);
+  s.chunks = 1;
+  const long long blocks = (long long)p.batch * p.heads * s.tiles;
+  const int row_tiles = std::max(1, ceil_div(p.nk, S::RT));
+  int per_chunk = row_tiles;
+  if (S::RW > 1 && blocks < 256) {
+    const int wanted = (int)std::min<long long>(ceil_div(512, blocks), ceil_div(row_tiles, 2));
+    per_chunk = ceil_div(row_tiles, std::max(1, wanted));
+    s.chunks = ceil_div(row_tiles, per_chunk);
+  }
+  s.chunk_rows = per_chunk * S::RT;
+  return s;
+}
+size_t part_bytes(const AttnLaunch &p, const Split &s) {
+  return s.chunks > 1 ? padded((size_t)s.chunks * p.batch * p.nq * p.heads * p.width * sizeof(float)) : 0;
+}
+size_t forward_bytes(const AttnLaunch &p, const Split &s) {
+  return s.chunks > 1 ? part_bytes(p, s) + padded((size_t)s.chunks * p.batch * p.nq * p.heads * 2 * sizeof(float)) : 0;
+}
+
+template <typename S>
+hipError_t forward_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  typedef typename S::Tag Tag;
+  Split s = plan_forward<S>(p);
+  if (bytes != nullptr) {
+    *bytes = forward_bytes(p, s);
+    return hipSuccess;
+  }
+  s.part = static_cast<float *>(p.workspace);
+  s.stats = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + part_bytes(p, s));
+  const long long blocks = (long long)p.batch * p.heads * s.tiles * s.chunks;
+  if (hipError_t e = run<S>(attn_forward_kernel<S>, blocks, stream, p, s)) return e;
+  if (s.chunks == 1) return hipSuccess;
+  const long long lanes = (long long)p.batch * p.nq * p.heads * (p.width / 4);
+  hipLaunchKernelGGL((attn_join_kernel<Tag>), dim3((unsigned)ceil_div(lanes, kThreads)), dim3(kThreads), 0, stream, p, s);
+  return hipGetLastError();
+}
+
+template <typename S>
+hipError_t grad_q_shape(const AttnLaunch &p, BackwardParts parts, hipStream_t stream) {
+  parts.tiles = ceil_div(p.nq, S::kColumns);
+  if (hipError_t e = run<S>(attn_grad_q_kernel<S>, (long long)p.batch * p.heads * parts.tiles, stream, p, parts)) return e;
+  if (parts.slopes == nullptr) return hipSuccess;
+  hipLaunchKernelGGL(attn_slope_grad_kernel, dim3(p.heads), dim3(kThreads), 0, stream, parts.slopes, p.grad_slopes, p.batch, p.heads, parts.tiles);
+  return hipGetLastError();
+}
+template <typename S>
+hipError_t grad_kv_shape(const AttnLaunch &p, BackwardParts parts, hipStream_t stream) {
+  parts.tiles = ceil_div(p.nk, S::kColumns);
+  return run<S>(attn_grad_kv_kernel<S>, (long long)p.batch * p.kv_heads * parts.tiles, stream, p, parts);
+}
+
+template <typename Tag, int W>
+hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  typedef Modes<Tag, W> M;
+  switch (column_mode((long long)p.batch * p.heads, p.nq)) {
+    case kWide2: return forward_shape<typename M::Wide2>(p, stream, bytes);
+    case kWide1: return forward_shape<typename M::Wide1>(p, stream, bytes);
+    default: return forward_shape<typename M::SplitRows>(p, stream, bytes);
+  }
+}
+size_t delta_bytes(const AttnLaunch &p) { return padded((size_t)p.batch * p.heads * p.nq * sizeof(float)); }
+
+template <typename Tag, int W>
+hipError_t backward_width(const AttnLaunch &p, hipStream_t stream) {
+  typedef Modes<Tag, W> M;
+  BackwardParts parts = {static_cast<float *>(p.workspace), nullptr, 0};
+  if (p.grad_slopes != nullptr) parts.slopes = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + delta_bytes(p));
+  hipError_t e = column_mode((long long)p.batch * p.heads, p.nq) == kSplitRows ? grad_q_shape<typename M::SplitRows>(p, parts, stream)
+                                                                               : grad_q_shape<typename M::Wide1>(p, parts, stream);
+  if (e != hipSuccess || (p.grad_k == nullptr && p.grad_v == nullptr)) return e;
+  return column_mode((long long)p.batch * p.kv_heads, p.nk) == kSplitRows ? grad_kv_shape<typename M::SplitRows>(p, parts, stream)
+                                                                          : grad_kv_shape<typename M::Wide1>(p, parts, stream);
+}
+
+template <typename Tag>
+hipError_t forward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  if (p.width <= 32) return forward_width<Tag, 32>(p, stream, bytes);
+  return p.width <= 64 ? forward_width<Tag, 64>(p, stream, bytes) : forward_width<Tag, 128>(p, stream, bytes);
+}
 template <typename Tag>
 hipError_t backward_t(const AttnLaunch &p, hipStream_t stream) {
-  float *delta = static_cast<float *>(p.workspace);
-  float *slope_part = p.grad_slopes != nullptr ? reinterpret_cast<float *>(static_cast<char *>(p.workspace) + rows_bytes(p)) : nullptr;
-  hipLaunchKernelGGL((attn_rows_grad_q_kernel<Tag>), dim3(row_blocks((long long)p.batch * p.nq * p.heads)), dim3(kRowThreads), 0, stream, p, delta, slope_part);
-  if (hipError_t e = hipGetLastError()) return e;
-  if (slope_part != nullptr) {
-    hipLaunchKernelGGL(attn_slope_grad_kernel, dim3(p.heads), dim3(kRowThreads), 0, stream, slope_part, p.grad_slopes, p.batch, p.heads, p.nq);
-    if (hipError_t e = hipGetLastError()) return e;
+  if (p.width <= 32) return backward_width<Tag, 32>(p, stream);
+  return p.width <= 64 ? backward_width<Tag, 64>(p, stream) : backward_width<Tag, 128>(p, stream);
+}
+hipError_t forward(int dtype, const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  switch (dtype) {
+    case F32::kCode: return forward_t<F32>(p, stream, bytes);
+    case F16::kCode: return forward_t<F16>(p, stream, bytes);
+    case BF16::kCode: return forward_t<BF16>(p, stream, bytes);
   }
-  hipLaunchKernelGGL((attn_rows_grad_kv_kernel<Tag>), dim3(row_blocks((long long)p.batch * p.nk * p.kv_heads)), dim3(kRowThreads), 0, stream, p, delta);
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
-size_t attn_forward_workspace_bytes(int, const AttnLaunch &) { return 0; }
-size_t attn_backward_workspace_bytes(int, const AttnLaunch &p) { return rows_bytes(p) * (p.slopes != nullptr ? 2 : 1); }
-
-hipError_t launch_attn_forward(int dtype, const AttnLaunch &p, hipStream_t stream) {
-  switch (dtype) {
-    case F32::kCode: return forward_t<F32>(p, stream);
-    case F16::kCode: return forward_t<F16>(p, stream);
-    case BF16::kCode: return forward_t<BF16>(p, stream);
-  }
-  return hipErrorInvalidValue;
+size_t attn_forward_workspace_bytes(int dtype, const AttnLaunch &p) {
+  size_t bytes = 0;
+  if (forward(dtype, p, nullptr, &bytes) != hipSuccess) return 0;      // the launch says why
+  return bytes;
 }
+size_t attn_backward_workspace_bytes(int, const AttnLaunch &p) {
+  // a part of the slopes' gradient for 16 columns or more
+  return delta_bytes(p) + (p.slopes != nullptr ? padded((size_t)p.batch * p.heads * ceil_div(p.nq, 16) * sizeof(float)) : 0);
+}
+
+hipError_t launch_attn_forward(int dtype, const AttnLaunch &p, hipStream_t stream) { return forward(dtype, p, stream, nullptr); }
 hipError_t launch_attn_backward(int dtype, const AttnLaunch &p, hipStream_t stream) {
   switch (dtype) {
     case F32::kCode: return backward_t<F32>(p, stream);

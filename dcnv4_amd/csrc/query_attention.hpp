@@ -19,7 +19,8 @@ struct AttnLaunch {
   const int *q_segments, *k_segments;             // (batch, tokens); no k_segments: all see all; no q_segments: zeros
   const float *q_points, *k_points, *slopes;      // (batch, tokens, 2), (heads,): all or none
   void *out;                                      // dense (batch, nq, heads, width)
-  float *lse;                                     // (batch, heads, nq): log of a row's sum; infinite where it sees nothing
+  void *out_rest;                                 // like out: what rounding took from it, for the backward of 16-bit types; or null
+  float *lse;                                     // (batch, heads, nq): base-2 log of a row's sum; infinite where it sees nothing
   // backward; gradients are dense and of the tensors' type
   AttnRows grad_out;
   void *grad_q, *grad_k, *grad_v;                 // null where not wanted
@@ -32,7 +33,7 @@ constexpr int kMaxAttnWidth = 128;
 size_t attn_forward_workspace_bytes(int dtype, const AttnLaunch &p);
 size_t attn_backward_workspace_bytes(int dtype, const AttnLaunch &p);
 hipError_t launch_attn_forward(int dtype, const AttnLaunch &p, hipStream_t stream);
-// Wants out and lse of the forward.
+// Wants out, out_rest and lse of the forward.
 hipError_t launch_attn_backward(int dtype, const AttnLaunch &p, hipStream_t stream);
 
 }  // namespace dcn

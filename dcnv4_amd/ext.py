@@ -329,17 +329,18 @@ def flash_deform_attn_backward_split(value, spatial_shapes, level_start_index, s
 
 
 def query_attention_forward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap):
-    """``[output, lse]`` of :func:`dcnv4_amd.functions.query_attention`, nothing left out: ``key_segments`` beside ``segments``,
-    positions of both beside ``slopes``; each of the five may be None.  ``lse`` (N, M, Lq) float32: the logarithm of a row's sum
-    of exponentials, infinite for a row that sees nothing."""
+    """``[output, rest, lse]`` of :func:`dcnv4_amd.functions.query_attention`, nothing left out: ``key_segments`` beside ``segments``,
+    positions of both beside ``slopes``; each of the five may be None.  ``rest``: what rounding took from the output, of its type
+    (None in float32); ``lse`` (N, M, Lq) float32: the base-2 logarithm of a row's sum of exponentials, infinite for a row that
+    sees nothing."""
     return _native.query_attention_forward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap)
 
 
-def query_attention_backward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap, output, lse,
-                             grad_output):
+def query_attention_backward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap, output, rest,
+                             lse, grad_output):
     """``[grad_query, grad_key, grad_value, grad_slopes]`` of :func:`query_attention_forward`; the last None without slopes."""
     return _native.query_attention_backward(query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap,
-                                            output, lse, grad_output)
+                                            output, rest, lse, grad_output)
 
 
 def add_layer_norm_forward(input, residual, weight, bias, eps, wide=False):

@@ -37,16 +37,17 @@ class QueryAttentionFunction(Function):
     @staticmethod
     def forward(ctx, query, key, value, segments, key_segments, positions, key_positions, slopes, scale, cap):
         args = (query, key, value, segments, key_segments, positions, key_positions, slopes)
-        output, lse = ext.query_attention_forward(*args, scale, cap)
-        ctx.save_for_backward(*args, output, lse)
+        output, rest, lse = ext.query_attention_forward(*args, scale, cap)
+        ctx.save_for_backward(*args, output, rest, lse)
         ctx.scalars = (scale, cap)
         return output
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output):
-        *args, output, lse = ctx.saved_tensors
-        grad_query, grad_key, grad_value, grad_slopes = ext.query_attention_backward(*args, *ctx.scalars, output, lse, grad_output)
+        *args, output, rest, lse = ctx.saved_tensors
+        grad_query, grad_key, grad_value, grad_slopes = ext.query_attention_backward(*args, *ctx.scalars, output, rest, lse,
+                                                                                           grad_output)
         return grad_query, grad_key, grad_value, None, None, None, None, grad_slopes, None, None
 
 
