@@ -24,7 +24,7 @@ struct AddNormLaunch {
   void *out, *sum;                // dense; the sum may be null
   int out_dtype, sum_dtype;
   float *stats;                   // (rows, 2): mean and 1 / deviation; the forward writes them where they are wanted
-  // backward: x and residual (or the sum, as x), stats, and
+  // backward: x, residual, stats and
   const void *grad_out, *grad_sum;                  // dense, of the outputs' types; grad_sum may be null
   void *grad_x, *grad_residual;                     // dense; grad_residual may be null
   int grad_x_dtype, grad_residual_dtype;

@@ -339,11 +339,10 @@ NormOutputs norm_forward(const NormInputs &a, bool want_sum, bool want_stats) {
   return o;
 }
 
-// Gradients of the two summands (one tensor for both where they have one type), weight and bias.  `a` holds the summands, or their
-// sum as x; the gradients have the types given.
-std::array<Tensor, 4> norm_backward(const NormInputs &a, const Tensor &stats, at::ScalarType sum_dtype, const Tensor &grad_out, const Tensor &grad_sum,
-                                    at::ScalarType x_dtype, at::ScalarType residual_dtype, std::array<bool, 4> want) {
+// Gradients of the two summands (one tensor for both where they have one type), weight and bias.
+std::array<Tensor, 4> norm_backward(const NormInputs &a, const Tensor &stats, const Tensor &grad_out, const Tensor &grad_sum, std::array<bool, 4> want) {
   norm_check(a);
+  const at::ScalarType sum_dtype = a.sum_dtype(), x_dtype = a.x.scalar_type(), residual_dtype = a.residual.defined() ? a.residual.scalar_type() : x_dtype;
   const int64_t width = a.x.size(-1), rows = a.x.numel() / width;
   check_beside(grad_out, "grad_output", a.x, a.wide ? at::kFloat : sum_dtype, a.x.sizes());
   if (grad_sum.defined()) check_beside(grad_sum, "grad_sum", a.x, sum_dtype, a.x.sizes());
@@ -377,27 +376,24 @@ std::array<Tensor, 4> norm_backward(const NormInputs &a, const Tensor &stats, at
   return grads;
 }
 
+// The summands are kept, not the sum: rounded to 16 bits it would show in the gradient of weight.
 struct AddLayerNormBackward final : torch::autograd::Node {
-  SavedVariable x, residual, weight, bias, sum;      // x and residual, or their sum where that is a result
+  SavedVariable x, residual, weight, bias;
   Tensor stats;
   float eps;
-  bool wide, keeps_sum, has_residual;
-  at::ScalarType sum_dtype, x_dtype, residual_dtype;
+  bool wide, has_residual;
+  at::ScalarType x_dtype, residual_dtype;
 
-  AddLayerNormBackward(const NormInputs &a, bool keeps_sum_)
-      : weight(a.weight, false), bias(a.bias, false), eps(a.eps), wide(a.wide), keeps_sum(keeps_sum_), has_residual(a.residual.defined()),
-        sum_dtype(a.sum_dtype()), x_dtype(a.x.scalar_type()), residual_dtype(has_residual ? a.residual.scalar_type() : x_dtype) {
-    if (keeps_sum) return;
-    x = SavedVariable(a.x, false);
-    if (has_residual) residual = SavedVariable(a.residual, false);
-  }
+  explicit AddLayerNormBackward(const NormInputs &a)
+      : x(a.x, false), residual(a.residual, false), weight(a.weight, false), bias(a.bias, false), eps(a.eps), wide(a.wide),
+        has_residual(a.residual.defined()), x_dtype(a.x.scalar_type()), residual_dtype(has_residual ? a.residual.scalar_type() : x_dtype) {}
   std::string name() const override { return "AddLayerNormFunctionBackward"; }
   void release_variables() override {
-    for (SavedVariable *s : {&x, &residual, &weight, &bias, &sum}) s->reset_data();
+    for (SavedVariable *s : {&x, &residual, &weight, &bias}) s->reset_data();
     stats = Tensor();
   }
   variable_list apply(variable_list &&grads) override {
-    const Tensor around = keeps_sum ? grads[1] : Tensor();
+    const Tensor around = grads.size() > 1 ? grads[1] : Tensor();
     if (!grads[0].defined() && !around.defined()) return variable_list(4);
     std::array<Tensor, 4> got;
     {
@@ -408,17 +404,13 @@ struct AddLayerNormBackward final : torch::autograd::Node {
         if (has_residual) got[1] = around.to(residual_dtype);
       } else {
         NormInputs a;
-        if (keeps_sum) {
-          a.x = sum.unpack(shared_from_this());
-        } else {
-          a.x = x.unpack();
-          if (has_residual) a.residual = residual.unpack();
-        }
+        a.x = x.unpack();
+        a.residual = residual.unpack();
         a.weight = weight.unpack();
         a.bias = bias.unpack();
         a.eps = eps;
         a.wide = wide;
-        got = norm_backward(a, stats, sum_dtype, dense(grads[0]), dense(around), x_dtype, residual_dtype,
+        got = norm_backward(a, stats, dense(grads[0]), dense(around),
                             {task_should_compute_output(0), has_residual && task_should_compute_output(1), task_should_compute_output(2),
                              task_should_compute_output(3)});
       }
@@ -453,13 +445,10 @@ PyObject *py_add_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const bool train = wants_grad({&in.x, &in.residual, &in.weight, &in.bias});
     o = norm_forward(in, want_sum, train);
     if (train) {
-      std::shared_ptr<AddLayerNormBackward> node(new AddLayerNormBackward(in, want_sum), torch::autograd::deleteNode);
+      std::shared_ptr<AddLayerNormBackward> node(new AddLayerNormBackward(in), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(in.x, in.residual, in.weight, in.bias));
       record(node, o.out);
-      if (want_sum) {
-        record(node, o.sum);
-        node->sum = SavedVariable(o.sum, true);
-      }
+      if (want_sum) record(node, o.sum);
       node->stats = o.stats;
     }
   }
@@ -489,8 +478,7 @@ PyObject *py_add_layer_norm_backward(PyObject *, PyObject *const *args, Py_ssize
   const Tensor around = a.optional_tensor();
   at::AutoGradMode no_grad(false);
   const bool residual = in.residual.defined();
-  const auto g = norm_backward(in, stats, in.sum_dtype(), grad, around, in.x.scalar_type(), residual ? in.residual.scalar_type() : in.x.scalar_type(),
-                               {true, residual, true, true});
+  const auto g = norm_backward(in, stats, grad, around, {true, residual, true, true});
   return Py_BuildValue("[NNNN]", wrapped(g[0]), wrapped(g[1]), wrapped(g[2]), wrapped(g[3]));
   END_HANDLE_TH_ERRORS
 }

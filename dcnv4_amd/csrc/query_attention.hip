@@ -18,6 +18,7 @@
 #include "query_attention.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "launch.hpp"
@@ -26,7 +27,7 @@
 namespace dcn {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave;
 constexpr float kInf = __builtin_inff(), kLog2e = 1.44269504088896340736f;
 constexpr int kHiddenColumn = -2;      // the segment of a column or query row that sees nothing; -1 is a padded key's
 
@@ -50,21 +51,26 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // A kernel's shape.  W: the width, zeros behind the tensors' own; RT: rows of a tile; RW: waves that share the columns and divide
-// a tile's rows, the others divide the columns; CF: sixteens of columns a wave.
-template <typename Tag_, int W_, int RT_, int RW_, int CF_>
+// a tile's rows, the others divide the columns; CF: sixteens of columns a wave; WAVES: of a workgroup.
+template <typename Tag_, int W_, int RT_, int RW_, int CF_, int WAVES_>
 struct Shape {
   typedef Tag_ Tag;
-  static constexpr int W = W_, RT = RT_, RW = RW_, CF = CF_;
+  static constexpr int W = W_, RT = RT_, RW = RW_, CF = CF_, kWaves = WAVES_, kThreads = kWaves * kWave;
   static constexpr int kSlices = W * Tag::kBytes / 64, kWidthBlocks = W / 16;
   static constexpr int kColumnWaves = kWaves / RW, kColumns = 16 * CF * kColumnWaves;
-  static constexpr int kRowBlocks = RT / RW / 16;                // of a wave in a tile
+  static constexpr int kRowBlocks = RT / RW / 16;                // of a wave in a tile, to work on
+  static constexpr int kCarried = RT / 16 / kWaves;              // and to bring into LDS
   static constexpr int kTensorBytes = RT * W * Tag::kBytes;
   // two tensors, then by row: segment, poison, position (2), logarithm, delta
   static constexpr int kSegments = 2 * kTensorBytes, kPoison = kSegments + RT * 4, kPoints = kPoison + RT * 4, kLse = kPoints + RT * 8,
                        kDelta = kLse + RT * 4, kTileBytes = kDelta + RT * 4;
-  static constexpr int kMergeBytes = RW > 1 ? kWaves * 16 * CF * (W + 4) * 4 + kWaves * 16 * CF * 8 : 0;
+  // sums of the waves that divide the rows: of the results, and four values a column
+  static constexpr int kMergeStats = kWaves * 16 * CF * (W + 4) * 4, kMergeBytes = RW > 1 ? kMergeStats + kWaves * 16 * CF * 16 : 0;
+  // two waves a SIMD at least, which also keeps the matrix instructions' results out of the accumulation registers and their copies;
+  // the largest tiles leave room for one
+  static constexpr int kWavesPerSimd = W * Tag::kBytes > 256 ? 1 : 2;
   static constexpr int kLdsBytes = std::max(2 * kTileBytes, kMergeBytes);
-  static_assert(kRowBlocks % 2 == 0 && kLdsBytes <= 156 * 1024);
+  static_assert(kRowBlocks % 2 == 0 && kCarried * kWaves * 16 == RT && kLdsBytes <= 156 * 1024);
 };
 
 // ---------------------------------------------------------------- a tile's way into LDS
@@ -83,14 +89,14 @@ __device__ __forceinline__ HeadRows head_rows(const AttnRows &t, int b, int head
 
 template <typename S>
 struct TileLoads {
-  u32x4 v[S::RT / 64][S::kSlices];
+  u32x4 v[S::kCarried][S::kSlices];
 
   __device__ __forceinline__ void request(const HeadRows &t, int row0, int rows, int width_bytes, int wave, int lane) {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(t.base + row0 * t.pitch, 0x7fffffffu);
     const int vec = (lane & 3) ^ ((lane >> 4) & 3);
 #pragma unroll
-    for (int u = 0; u < S::RT / 64; ++u) {
-      const int row = (wave + 4 * u) * 16 + lane / 4;
+    for (int u = 0; u < S::kCarried; ++u) {
+      const int row = (wave + S::kWaves * u) * 16 + lane / 4;
       const uint32_t at = (uint32_t)row * (uint32_t)t.pitch + (uint32_t)vec * 16;
 #pragma unroll
       for (int s = 0; s < S::kSlices; ++s)
@@ -99,10 +105,10 @@ struct TileLoads {
   }
   __device__ __forceinline__ void put(char *tensor, int wave, int lane) const {
 #pragma unroll
-    for (int u = 0; u < S::RT / 64; ++u)
+    for (int u = 0; u < S::kCarried; ++u)
 #pragma unroll
       for (int s = 0; s < S::kSlices; ++s)
-        *reinterpret_cast<u32x4 *>(tensor + s * S::RT * 64 + (wave + 4 * u) * 1024 + lane * 16) = v[u][s];
+        *reinterpret_cast<u32x4 *>(tensor + s * S::RT * 64 + (wave + S::kWaves * u) * 1024 + lane * 16) = v[u][s];
   }
   // Clears vectors that hold an infinity or NaN; whether the lane's row u had one.
   __device__ __forceinline__ bool clear_bad(int u) {
@@ -128,7 +134,7 @@ template <typename S>
 __device__ __forceinline__ void put_poison(char *tile, int u, bool bad, int wave, int lane) {
   const uint64_t all = __ballot(bad);
   if ((lane & 3) == 0)
-    reinterpret_cast<float *>(tile + S::kPoison)[(wave + 4 * u) * 16 + lane / 4] = (all >> lane & 15) != 0 ? __builtin_nanf("") : 0.f;
+    reinterpret_cast<float *>(tile + S::kPoison)[(wave + S::kWaves * u) * 16 + lane / 4] = (all >> lane & 15) != 0 ? __builtin_nanf("") : 0.f;
 }
 
 template <typename S>
@@ -201,25 +207,59 @@ __device__ __forceinline__ float dot_16_bytes(u32x4 a, u32x4 b, float sum) {
 // Scores go into exp2, so they are in units of its exponent.  Without cap and distance that is one factor, which rides along where
 // the maximum is taken off.
 struct Scores {
-  float cap, scale, tanh_scale, factor, slope;
-  bool bent, apart;      // there is a cap; a distance
-  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : cap(p.cap), scale(p.scale), bent(p.cap > 0.f), apart(p.slopes != nullptr) {
-    tanh_scale = bent ? scale / cap : 0.f;
-    factor = (bent ? cap : scale) * kLog2e;
+  float tanh_scale, factor, slope;
+  bool bent, apart, scaled;      // there is a cap; a distance; neither, but a factor that cannot ride along
+  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : bent(p.cap > 0.f), apart(p.slopes != nullptr) {
+    tanh_scale = bent ? p.scale / p.cap : 0.f;
+    factor = (bent ? p.cap : p.scale) * kLog2e;
     slope = apart ? p.slopes[head] * kLog2e : 0.f;
+    scaled = !bent && (apart || !(p.scale > 0.f));      // products stand for scores in the order of their size
   }
-  // the products as they come may stand for the scores, in the order of their size
-  __device__ __forceinline__ bool as_they_are() const { return !bent && !apart && scale > 0.f; }
-  template <typename Tag>
-  __device__ __forceinline__ float tanh_of(float product) const {
-    const float x = product * tanh_scale;
-    if constexpr (Tag::kBytes == 4) return tanhf(x);      // fp32 results see the last bits
-    else return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * kLog2e)) + 1.f), 1.f);
-  }
+  __device__ __forceinline__ bool as_they_are() const { return !bent && !scaled; }
 };
 __device__ __forceinline__ float distance(f32x2 a, f32x2 b) {
   const float x = a.x - b.x, y = a.y - b.y;
   return __builtin_amdgcn_sqrtf(fmaf(x, x, y * y));
+}
+
+// Scores of N blocks of 16 rows, from the products in s; point_of(n, r): the rows' positions.  With GRADS also the distances and
+// 1 - tanh^2.  What a call has is the same for all lanes: a loop for each, not a question for each score.
+template <typename Tag, bool GRADS, int N, int CF, typename Points>
+__device__ __forceinline__ void finish_scores(const Scores &scores, f32x4 (&s)[N][CF], f32x4 (&far)[GRADS ? N : 1][CF], f32x4 (&bend)[GRADS ? N : 1][CF],
+                                              const f32x2 (&point)[CF], Points point_of) {
+  if (scores.bent) {
+    const float rate = scores.tanh_scale * (2.f * kLog2e);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int f = 0; f < CF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float t;
+          if constexpr (Tag::kBytes == 4) t = tanhf(s[n][f][r] * scores.tanh_scale);      // fp32 results see the last bits
+          else t = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][f][r] * rate) + 1.f), 1.f);
+          if constexpr (GRADS) bend[n][f][r] = fmaf(-t, t, 1.f);
+          s[n][f][r] = t * scores.factor;
+        }
+  }
+  if (scores.scaled)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int f = 0; f < CF; ++f) s[n][f] *= scores.factor;
+  if (scores.apart)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x2 there = point_of(n, r);
+#pragma unroll
+        for (int f = 0; f < CF; ++f) {
+          const float d = distance(point[f], there);
+          if constexpr (GRADS) far[n][f][r] = d;
+          s[n][f][r] = fmaf(-scores.slope, d, s[n][f][r]);
+        }
+      }
 }
 
 // ---------------------------------------------------------------- which tiles
@@ -263,7 +303,7 @@ struct TileMasks {
   uint64_t some, every;      // bit t: tile t of up to 64
 };
 // Rows first .. last - 1; all waves together.  flags: 64 bytes of LDS, free again behind the next barrier.
-template <int RT, bool KEYS>
+template <int RT, int WAVES, bool KEYS>
 __device__ __forceinline__ TileMasks tile_masks(const int *row_segments, bool masked, const ColumnRange &c, int first, int last, char *flags, int wave, int lane) {
   const int tiles = min(64, (last - first + RT - 1) / RT);
   if (!masked) {
@@ -272,14 +312,25 @@ __device__ __forceinline__ TileMasks tile_masks(const int *row_segments, bool ma
     m.every = first + tiles * RT <= last ? m.some : m.some >> 1;
     return m;
   }
-  for (int t = wave; t < tiles; t += kWaves) {
+  // a wave's tiles all at once: their loads are one wait
+  constexpr int kMine = 64 / WAVES, kParts = RT / 64;
+  int v[kMine][kParts];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i)
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      const int row = first + (wave + i * WAVES) * RT + u * 64 + lane;
+      v[i][u] = row < last ? (row_segments != nullptr ? row_segments[row] : 0) : kHiddenColumn;
+    }
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int t = wave + i * WAVES;
+    if (t >= tiles) break;
     bool some = false, every = true;
 #pragma unroll
-    for (int u = 0; u < RT / 64; ++u) {
-      const int row = first + t * RT + u * 64 + lane;
-      const int v = row < last ? (row_segments != nullptr ? row_segments[row] : 0) : kHiddenColumn;
-      some = some || some_pair<KEYS>(c, v);
-      every = every && row < last && every_pair<KEYS>(c, v);
+    for (int u = 0; u < kParts; ++u) {
+      some = some || some_pair<KEYS>(c, v[i][u]);
+      every = every && first + t * RT + u * 64 + lane < last && every_pair<KEYS>(c, v[i][u]);
     }
     const uint64_t has = __ballot(some), all = __ballot(every);
     if (lane == 0) flags[t] = (char)((has != 0) | (all == ~0ull) << 1);
@@ -296,38 +347,30 @@ struct RowLoads {
   float lse, delta;
 };
 
-// Walks the tiles: request(row0) starts the loads of a tile, put(tile, row0, every) brings what came into LDS, work(tile, every) computes.
-// A tile's loads are under way while the one before is worked on; two tiles of LDS in turn, one barrier a tile.
+// Walks the tiles: request(row0) starts the loads of a tile, put(tile, every) brings what came into LDS, work(tile, every) computes.
+// A tile's loads are under way while the one before is worked on (two ahead gained nothing); two tiles of LDS in turn, one barrier a tile.
 template <typename S, bool KEYS, typename Request, typename Put, typename Work>
 __device__ __forceinline__ void walk_tiles(const int *row_segments, bool masked, const ColumnRange &c, int first, int last, char *lds, char *flags, int wave,
                                            int lane, Request request, Put put, Work work) {
   for (int window = first; window < last; window += 64 * S::RT) {
-    TileMasks m = tile_masks<S::RT, KEYS>(row_segments, masked, c, window, last, flags, wave, lane);
+    TileMasks m = tile_masks<S::RT, S::kWaves, KEYS>(row_segments, masked, c, window, last, flags, wave, lane);
     if (m.some != 0) {
-      auto take = [&](bool &every) {
+      bool every = false;
+      auto next = [&] {
         const int t = __builtin_ctzll(m.some);
         m.some &= m.some - 1;
         every = m.every >> t & 1;
-        return window + t * S::RT;
+        request(window + t * S::RT);
       };
-      bool every;
-      int row0 = take(every), turn = 0;
-      request(row0);
-      put(lds, row0, every);
-      __syncthreads();
-      for (;;) {
-        const bool more = m.some != 0;
-        bool next_every = false;
-        if (more) {
-          row0 = take(next_every);
-          request(row0);
-        }
-        work(lds + turn * S::kTileBytes, every);
-        if (!more) break;
-        turn ^= 1;
-        every = next_every;
-        put(lds + turn * S::kTileBytes, row0, every);
+      next();
+      for (int turn = 0;; turn ^= 1) {
+        char *tile = lds + turn * S::kTileBytes;
+        const bool whole = every, more = m.some != 0;
+        put(tile, whole);
         __syncthreads();
+        if (more) next();
+        work(tile, whole);
+        if (!more) break;
       }
     }
     __syncthreads();
@@ -394,11 +437,11 @@ __device__ __forceinline__ f32x4 rounded_off(f32x4 v) {
 // ---------------------------------------------------------------- forward
 struct Split {
   int tiles, chunks, chunk_rows;      // column tiles of a head; parts of the rows, a whole number of tiles each
-  float *part, *stats;                // [chunk][batch][query][head][width], [..][2]: unnormalised sums, maximum and sum
+  float *part, *stats;                // [chunk][batch][query][head][width], [..][4]: unnormalised sums; maximum, sum, exact sum
 };
 
 template <typename S>
-__global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch p, const Split split) {
+__global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_kernel(const AttnLaunch p, const Split split) {
   typedef typename S::Tag Tag;
   extern __shared__ __align__(16) char lds[];
   __shared__ char s_flags[64];
@@ -429,11 +472,15 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
   }
   const ColumnRange range = masked ? column_range<false>(q_segments, column0, p.nq, S::kColumns, lane) : ColumnRange{};
 
+  // total: sums of the weights as the product takes them, rounded, which divide the result; exact: of the weights themselves, for the
+  // logarithm from which the backward forms them again
   f32x4 acc[S::kWidthBlocks][S::CF], total[S::CF];
-  float top[S::CF];
+  float top[S::CF], exact[S::CF];
+  const bool train = Tag::kBytes == 2 && p.lse != nullptr;
 #pragma unroll
   for (int f = 0; f < S::CF; ++f) {
     top[f] = -kInf;
+    exact[f] = 0.f;
     total[f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -450,10 +497,10 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
       if (scores.apart) next.point = row < last ? reinterpret_cast<const f32x2 *>(p.k_points)[(long long)at.b * p.nk + row] : f32x2{0.f, 0.f};
     }
   };
-  auto put = [&](char *tile, int, bool every) {
+  auto put = [&](char *tile, bool every) {
     if (!every)
 #pragma unroll
-      for (int u = 0; u < S::RT / 64; ++u) put_poison<S>(tile, u, next_v.clear_bad(u), wave, lane);
+      for (int u = 0; u < S::kCarried; ++u) put_poison<S>(tile, u, next_v.clear_bad(u), wave, lane);
     next_k.put(tile, wave, lane);
     next_v.put(tile + S::kTensorBytes, wave, lane);
     if ((int)threadIdx.x < S::RT) {
@@ -475,22 +522,9 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
         for (int f = 0; f < S::CF; ++f) s[n][f] = mfma_64_bytes<Tag>(a, q[f][sl], s[n][f]);
       }
     }
-    if (!plain)
-#pragma unroll
-      for (int n = 0; n < S::kRowBlocks; ++n) {
-        const f32x2 *from = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + (block0 + n) * 16 + 4 * g;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          f32x2 other = {0.f, 0.f};
-          if (scores.apart) other = from[r];
-#pragma unroll
-          for (int f = 0; f < S::CF; ++f) {
-            float v = (scores.bent ? scores.tanh_of<Tag>(s[n][f][r]) : s[n][f][r]) * scores.factor;
-            if (scores.apart) v = fmaf(-scores.slope, distance(point[f], other), v);
-            s[n][f][r] = v;
-          }
-        }
-      }
+    const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block0 * 16 + 4 * g;
+    f32x4 unused[1][S::CF];
+    finish_scores<Tag, false, S::kRowBlocks, S::CF>(scores, s, unused, unused, point, [&](int n, int r) { return points[n * 16 + r]; });
     if (!every)
 #pragma unroll
       for (int n = 0; n < S::kRowBlocks; ++n) {
@@ -520,19 +554,28 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
 #pragma unroll
         for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] *= keep;
         total[f] *= keep;
+        exact[f] *= keep;
       }
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      const float off = kForwardShift<Tag> - (top[f] == -kInf ? 0.f : top[f]);
+#pragma unroll
+      for (int n = 0; n < S::kRowBlocks; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[n][f][r] = __builtin_amdgcn_exp2f(fmaf(s[n][f][r], factor, off));
+    }
+    if (Tag::kBytes == 4 || train)
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+        for (int n = 0; n < S::kRowBlocks; ++n) exact[f] += (s[n][f].x + s[n][f].y) + (s[n][f].z + s[n][f].w);
 #pragma unroll
     for (int n = 0; n < S::kRowBlocks; n += 2) {
       f32x4 w[2][S::CF];
 #pragma unroll
       for (int f = 0; f < S::CF; ++f) {
-        const float off = kForwardShift<Tag> - (top[f] == -kInf ? 0.f : top[f]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) w[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[n + h][f][r], factor, off));
-          if constexpr (Tag::kBytes == 4) total[f] += w[h][f];
-        }
+        w[0][f] = s[n][f];
+        w[1][f] = s[n + 1][f];
         if constexpr (Tag::kBytes == 2) {      // of the weights as the product takes them
           constexpr uint32_t one = Tag::kCode == F16::kCode ? 0x3c003c00u : 0x3f803f80u;
           const float v[8] = {w[0][f].x, w[0][f].y, w[0][f].z, w[0][f].w, w[1][f].x, w[1][f].y, w[1][f].z, w[1][f].w};
@@ -547,20 +590,21 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
   float sum[S::CF];
 #pragma unroll
   for (int f = 0; f < S::CF; ++f) {
-    sum[f] = Tag::kBytes == 4 ? column_sum((total[f].x + total[f].y) + (total[f].z + total[f].w)) : total[f].x;
+    exact[f] = column_sum(exact[f]);
+    sum[f] = Tag::kBytes == 4 ? exact[f] : total[f].x;
     if (segment[f] < 0) {      // sees nothing
-      sum[f] = 0.f;
+      sum[f] = exact[f] = 0.f;
       top[f] = -kInf;
 #pragma unroll
       for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
   if constexpr (S::RW > 1) {
-    f32x2 *s_stats = reinterpret_cast<f32x2 *>(lds + kWaves * 16 * S::CF * (S::W + 4) * 4);
+    f32x4 *s_stats = reinterpret_cast<f32x4 *>(lds + S::kMergeStats);
     auto slot = [&](int w, int f) { return ((w * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c; };
 #pragma unroll
     for (int f = 0; f < S::CF; ++f)
-      if (g == 0) s_stats[slot(row_wave, f)] = f32x2{top[f], sum[f]};
+      if (g == 0) s_stats[slot(row_wave, f)] = f32x4{top[f], sum[f], exact[f], 0.f};
     __syncthreads();
 #pragma unroll
     for (int f = 0; f < S::CF; ++f) {
@@ -569,9 +613,14 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
 #pragma unroll
       for (int w = 0; w < S::RW; ++w) now = fmaxf(now, s_stats[slot(w, f)].x);
       const float base = now == -kInf ? 0.f : now;
-      sum[f] = 0.f;
+      sum[f] = exact[f] = 0.f;
 #pragma unroll
-      for (int w = 0; w < S::RW; ++w) sum[f] = fmaf(s_stats[slot(w, f)].y, __builtin_amdgcn_exp2f(s_stats[slot(w, f)].x - base), sum[f]);
+      for (int w = 0; w < S::RW; ++w) {
+        const f32x4 of = s_stats[slot(w, f)];
+        const float keep = __builtin_amdgcn_exp2f(of.x - base);
+        sum[f] = fmaf(of.y, keep, sum[f]);
+        exact[f] = fmaf(of.z, keep, exact[f]);
+      }
       const float keep = __builtin_amdgcn_exp2f(was - base);
       top[f] = now;
 #pragma unroll
@@ -600,40 +649,48 @@ __global__ void __launch_bounds__(kThreads) attn_forward_kernel(const AttnLaunch
       }
     }
     if (g != 0 || row_wave != 0) continue;
-    if (split_rows) reinterpret_cast<f32x2 *>(split.stats)[part_row] = f32x2{top[f], sum[f]};
+    if (split_rows) reinterpret_cast<f32x4 *>(split.stats)[part_row] = f32x4{top[f], sum[f], exact[f], 0.f};
     else if (p.lse != nullptr)
-      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = sum[f] == 0.f ? kInf : top[f] - kForwardShift<Tag> + __builtin_amdgcn_logf(sum[f]);
+      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = exact[f] == 0.f ? kInf : top[f] - kForwardShift<Tag> + __builtin_amdgcn_logf(exact[f]);
   }
 }
 
-// The chunks of a row: a lane takes four elements.
+// The chunks of a row: a wave each, a lane four elements of every (64 / lanes)th chunk.  Lanes a row: a power of two.
 template <typename Tag>
-__global__ void __launch_bounds__(kThreads) attn_join_kernel(const AttnLaunch p, const Split split) {
-  const int lanes = p.width / 4;
-  const long long rows = (long long)p.batch * p.nq * p.heads, id = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = id / lanes;
-  const int column = (int)(id % lanes) * 4;
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnLaunch p, const Split split, int lanes) {
+  const int lane = threadIdx.x % kWave, teams = kWave / lanes, team = lane / lanes, column = lane % lanes * 4;
+  const long long rows = (long long)p.batch * p.nq * p.heads, row = (long long)blockIdx.x * kJoinWaves + threadIdx.x / kWave;
   if (row >= rows) return;
-  const f32x2 *stats = reinterpret_cast<const f32x2 *>(split.stats);
+  const f32x4 *stats = reinterpret_cast<const f32x4 *>(split.stats);
   float top = -kInf;
-  for (int k = 0; k < split.chunks; ++k) top = fmaxf(top, stats[k * rows + row].x);
+  for (int k = lane; k < split.chunks; k += kWave) top = fmaxf(top, stats[k * rows + row].x);
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
   const float base = top == -kInf ? 0.f : top;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
+  float sum = 0.f, exact = 0.f;
 #pragma unroll 4
-  for (int k = 0; k < split.chunks; ++k) {
-    const f32x2 s = stats[k * rows + row];
+  for (int k = team; k < split.chunks; k += teams) {
+    const f32x4 s = stats[k * rows + row];
     const float w = __builtin_amdgcn_exp2f(s.x - base);
-    const f32x4 v = *reinterpret_cast<const f32x4 *>(split.part + (k * rows + row) * p.width + column);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (column < p.width) v = *reinterpret_cast<const f32x4 *>(split.part + (k * rows + row) * p.width + column);
     sum = fmaf(w, s.y, sum);
+    exact = fmaf(w, s.z, exact);
     acc += v * w;
   }
+  for (int o = lanes; o < kWave; o <<= 1) {
+    sum += __shfl_xor(sum, o, kWave);
+    exact += __shfl_xor(exact, o, kWave);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, kWave);
+  }
+  if (team != 0 || column >= p.width) return;
   acc *= sum == 0.f ? 0.f : 1.f / sum;
   store4<Tag>(p.out, row * p.width + column, acc);
   if (p.out_rest != nullptr) store4<Tag>(p.out_rest, row * p.width + column, rounded_off<Tag>(acc));
   if (p.lse != nullptr && column == 0) {
     const long long head = row % p.heads, i = row / p.heads % p.nq, b = row / p.heads / p.nq;
-    p.lse[(b * p.heads + head) * p.nq + i] = sum == 0.f ? kInf : top - kForwardShift<Tag> + __builtin_amdgcn_logf(sum);
+    p.lse[(b * p.heads + head) * p.nq + i] = exact == 0.f ? kInf : top - kForwardShift<Tag> + __builtin_amdgcn_logf(exact);
   }
 }
 
@@ -681,50 +738,34 @@ struct ColumnScale {
   }
 };
 
-// Scores of 32 rows, from the products: rows' positions in `other`.  far, bend: the distances and 1 - tanh^2, for the gradients.
-template <typename S, typename Points>
-__device__ __forceinline__ void finish_scores(const Scores &scores, f32x4 (&s)[2][S::CF], f32x4 (&far)[2][S::CF], f32x4 (&bend)[2][S::CF],
-                                              const f32x2 (&point)[S::CF], Points other) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      f32x2 there = {0.f, 0.f};
-      if (scores.apart) there = other(h, r);
-#pragma unroll
-      for (int f = 0; f < S::CF; ++f) {
-        float v = s[h][f][r];
-        if (scores.bent) {
-          v = scores.tanh_of<typename S::Tag>(v);
-          bend[h][f][r] = fmaf(-v, v, 1.f);
-        }
-        v *= scores.factor;
-        if (scores.apart) {
-          far[h][f][r] = distance(point[f], there);
-          v = fmaf(-scores.slope, far[h][f][r], v);
-        }
-        s[h][f][r] = v;
-      }
-    }
-}
-
 struct BackwardParts {
   float *delta, *slopes;      // (batch, heads, queries); (batch, heads, column tiles)
-  int tiles;
+  int tiles;                  // column tiles of a head
+  // Few columns: the rows, and heads that share a key head, are divided among workgroups; parts [chunk][token][head][width] in fp32 are
+  // added behind.
+  int chunks, chunk_rows, head_parts;
+  float *part;
 };
+// Where a chunk's results go.
+template <typename Tag>
+__device__ __forceinline__ void store_grad(void *grad, float *part, size_t chunk_rows_before, size_t row, int width, int column, f32x4 v) {
+  if (part != nullptr) *reinterpret_cast<f32x4 *>(part + (chunk_rows_before + row) * width + column) = v;
+  else if (grad != nullptr) store4<Tag>(grad, row * width + column, v);
+}
 
 // dQ, delta and the slopes' parts: columns are queries, rows keys.
 template <typename S>
-__global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnLaunch p, const BackwardParts parts) {
+__global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_kernel(const AttnLaunch p, const BackwardParts parts) {
   typedef typename S::Tag Tag;
   extern __shared__ __align__(16) char lds[];
   __shared__ char s_flags[64];
-  __shared__ float s_slopes[kWaves];
+  __shared__ float s_slopes[S::kWaves];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
   const int row_wave = wave / S::kColumnWaves, column_wave = wave % S::kColumnWaves;
-  const Place at(p.heads, parts.tiles, 1);
+  const Place at(p.heads, parts.tiles, parts.chunks);
   const int kv = at.head / (p.heads / p.kv_heads), width_bytes = p.width * Tag::kBytes;
   const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
+  const int first = at.chunk * parts.chunk_rows, last = min(p.nk, first + parts.chunk_rows);
   const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
   const Scores scores(p, at.head);
   const bool plain = scores.as_they_are(), masked = p.k_segments != nullptr;
@@ -767,7 +808,7 @@ __global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnLaunch 
     if (scores.apart && i < p.nq) point[f] = reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + i];
     lse[f] = i < p.nq ? p.lse[stat] : kInf;
     delta[f] = column_sum(delta[f]);
-    if (i < p.nq && g == 0 && row_wave == 0) parts.delta[stat] = delta[f];
+    if (i < p.nq && g == 0 && row_wave == 0 && at.chunk == 0) parts.delta[stat] = delta[f];
   }
   const ColumnRange range = masked ? column_range<false>(q_segments, column0, p.nq, S::kColumns, lane) : ColumnRange{};
 
@@ -777,25 +818,29 @@ __global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnLaunch 
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   ColumnScale<S> up;
-  float slope[S::CF];
+  // The slopes' gradient is fp32 and a sum of terms that nearly cancel in each row: delta, which is as exact as the forward's weights
+  // were rounded, would show.  With w the weights formed here, a row adds -sum w (t - mean) distance, mean = sum w t / sum w: four
+  // sums a column, over w (t - delta) = dS for t to keep them small.  Sums of w, w distance, dS, dS distance:
+  const bool want_slopes = parts.slopes != nullptr;
+  f32x4 moment[S::CF];
 #pragma unroll
-  for (int f = 0; f < S::CF; ++f) slope[f] = 0.f;
+  for (int f = 0; f < S::CF; ++f) moment[f] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   TileLoads<S> next_k, next_v;
   RowLoads next = {};
   auto request = [&](int row0) {
-    next_k.request(keys, row0, p.nk, width_bytes, wave, lane);
-    next_v.request(values, row0, p.nk, width_bytes, wave, lane);
+    next_k.request(keys, row0, last, width_bytes, wave, lane);
+    next_v.request(values, row0, last, width_bytes, wave, lane);
     const int row = row0 + (int)threadIdx.x;
     if ((int)threadIdx.x < S::RT) {
-      next.segment = row < p.nk ? (masked ? k_segments[row] : 0) : -1;
-      if (scores.apart) next.point = row < p.nk ? reinterpret_cast<const f32x2 *>(p.k_points)[(long long)at.b * p.nk + row] : f32x2{0.f, 0.f};
+      next.segment = row < last ? (masked ? k_segments[row] : 0) : -1;
+      if (scores.apart) next.point = row < last ? reinterpret_cast<const f32x2 *>(p.k_points)[(long long)at.b * p.nk + row] : f32x2{0.f, 0.f};
     }
   };
-  auto put = [&](char *tile, int, bool every) {
+  auto put = [&](char *tile, bool every) {
     if (!every)
 #pragma unroll
-      for (int u = 0; u < S::RT / 64; ++u) put_poison<S>(tile, u, next_k.clear_bad(u), wave, lane);
+      for (int u = 0; u < S::kCarried; ++u) put_poison<S>(tile, u, next_k.clear_bad(u), wave, lane);
     next_k.put(tile, wave, lane);
     next_v.put(tile + S::kTensorBytes, wave, lane);
     if ((int)threadIdx.x < S::RT) {
@@ -823,54 +868,65 @@ __global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnLaunch 
         }
       }
       const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
-      if (!plain) finish_scores<S>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
+      finish_scores<Tag, true, 2, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
       const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
       const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int f = 0; f < S::CF; ++f) {
-            float x = s[h][f][r];
-            if (!every) x += poison[h * 16 + r];
-            float ds = __builtin_amdgcn_exp2f(fmaf(x, factor, -lse[f])) * (t[h][f][r] - delta[f]);
-            if (!every) ds = segments[h * 16 + r] == 0 || segments[h * 16 + r] == segment[f] ? ds : 0.f;
-            s[h][f][r] = ds;
-          }
-      if (scores.apart)
+      if (!every)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int f = 0; f < S::CF; ++f) {
-              // a distance to a place that is not seen may be anything
-              const float apart = every || s[h][f][r] != 0.f ? far[h][f][r] : 0.f;
-              slope[f] = fmaf(-s[h][f][r], apart, slope[f]);
+              const bool seen = segments[h * 16 + r] == 0 || segments[h * 16 + r] == segment[f];
+              s[h][f][r] = seen ? s[h][f][r] + poison[h * 16 + r] : -kInf;
+              // what else there is of a pair that is not seen may be anything
+              t[h][f][r] = seen ? t[h][f][r] : delta[f];
+              if (scores.apart) far[h][f][r] = seen ? far[h][f][r] : 0.f;
+              if (scores.bent) bend[h][f][r] = seen ? bend[h][f][r] : 0.f;
             }
-      if (scores.bent)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) {
+            s[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[h][f][r], factor, -lse[f]));
+            t[h][f][r] = s[h][f][r] * (t[h][f][r] - delta[f]);
+          }
+      if (want_slopes)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int f = 0; f < S::CF; ++f)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[h][f][r] = every || s[h][f][r] != 0.f ? s[h][f][r] * bend[h][f][r] : 0.f;
-      up.apply(s, acc);
-      add_product<S>(acc, tile, block, s, lane);
+            for (int r = 0; r < 4; ++r) {
+              moment[f].x += s[h][f][r];
+              moment[f].y = fmaf(s[h][f][r], far[h][f][r], moment[f].y);
+              moment[f].z += t[h][f][r];
+              moment[f].w = fmaf(t[h][f][r], far[h][f][r], moment[f].w);
+            }
+      if (scores.bent)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) t[h][f] *= bend[h][f];
+      up.apply(t, acc);
+      add_product<S>(acc, tile, block, t, lane);
     }
   };
-  walk_tiles<S, false>(k_segments, masked, range, 0, p.nk, lds, s_flags, wave, lane, request, put, work);
+  walk_tiles<S, false>(k_segments, masked, range, first, last, lds, s_flags, wave, lane, request, put, work);
 
 #pragma unroll
   for (int f = 0; f < S::CF; ++f) {
     const float by = p.scale / up.by[f];
     const bool sees = segment[f] >= 0;
-    if (!sees) slope[f] = 0.f;
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = sees ? acc[d][f] * by : f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!sees) moment[f] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   merge_rows<S>(acc, lds, row_wave, column_wave, lane);
+  const size_t rows_before = (size_t)at.chunk * p.batch * p.nq * p.heads;
   if (p.grad_q != nullptr)
 #pragma unroll
     for (int f = 0; f < S::CF; ++f) {
@@ -879,29 +935,57 @@ __global__ void __launch_bounds__(kThreads) attn_grad_q_kernel(const AttnLaunch 
       const size_t row = ((size_t)at.b * p.nq + i) * p.heads + at.head;
 #pragma unroll
       for (int d = 0; d < S::kWidthBlocks; ++d)
-        if (holds<S>(d, row_wave) && d * 16 + g * 4 < p.width) store4<Tag>(p.grad_q, row * p.width + d * 16 + g * 4, acc[d][f]);
+        if (holds<S>(d, row_wave) && d * 16 + g * 4 < p.width)
+          store_grad<Tag>(p.grad_q, parts.part, rows_before, row, p.width, d * 16 + g * 4, acc[d][f]);
     }
-  if (parts.slopes != nullptr) {
+  if (want_slopes) {
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) moment[f][e] = column_sum(moment[f][e]);
+    if constexpr (S::RW > 1) {
+      f32x4 *s_stats = reinterpret_cast<f32x4 *>(lds + S::kMergeStats);
+      auto slot = [&](int w, int f) { return ((w * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c; };
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f)
+        if (g == 0) s_stats[slot(row_wave, f)] = moment[f];
+      __syncthreads();
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) {
+        moment[f] = s_stats[slot(0, f)];
+#pragma unroll
+        for (int w = 1; w < S::RW; ++w) moment[f] += s_stats[slot(w, f)];
+      }
+    }
     float sum = 0.f;
 #pragma unroll
-    for (int f = 0; f < S::CF; ++f) sum += slope[f];
+    for (int f = 0; f < S::CF; ++f)
+      if (g == 0 && row_wave == 0 && mine0 + 16 * f + c < p.nq && moment[f].x != 0.f)
+        sum -= (moment[f].w - moment[f].z / moment[f].x * moment[f].y) / moment[f].x;
     sum = cluster_sum(sum, kWave);
     if (lane == 0) s_slopes[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) parts.slopes[((size_t)at.b * p.heads + at.head) * parts.tiles + at.tile] = (s_slopes[0] + s_slopes[1]) + (s_slopes[2] + s_slopes[3]);
+    if (threadIdx.x == 0) {
+      sum = s_slopes[0];
+#pragma unroll
+      for (int w = 1; w < S::kWaves; ++w) sum += s_slopes[w];
+      parts.slopes[((size_t)at.b * p.heads + at.head) * parts.tiles + at.tile] = sum;
+    }
   }
 }
 
 // dK and dV: columns are keys, rows the queries of every head that shares the key head.
 template <typename S>
-__global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch p, const BackwardParts parts) {
+__global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_kernel(const AttnLaunch p, const BackwardParts parts) {
   typedef typename S::Tag Tag;
   extern __shared__ __align__(16) char lds[];
   __shared__ char s_flags[64];
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, g = lane >> 4, c = lane & 15;
   const int row_wave = wave / S::kColumnWaves, column_wave = wave % S::kColumnWaves;
-  const Place at(p.kv_heads, parts.tiles, 1);
-  const int share = p.heads / p.kv_heads, width_bytes = p.width * Tag::kBytes;
+  const Place at(p.kv_heads, parts.tiles, parts.chunks);
+  const int share = p.heads / p.kv_heads, heads_here = share / parts.head_parts, head0 = at.head * share + at.chunk % parts.head_parts * heads_here;
+  const int first = at.chunk / parts.head_parts * parts.chunk_rows, last = min(p.nq, first + parts.chunk_rows);
+  const int width_bytes = p.width * Tag::kBytes;
   const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
   const bool masked = p.k_segments != nullptr;
 
@@ -931,7 +1015,7 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch
     for (int d = 0; d < S::kWidthBlocks; ++d) dk[d][f] = dv[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   ColumnScale<S> up;
 
-  for (int head = at.head * share; head < (at.head + 1) * share; ++head) {
+  for (int head = head0; head < head0 + heads_here; ++head) {
     const HeadRows queries = head_rows<Tag>(p.q, at.b, head), grads = head_rows<Tag>(p.grad_out, at.b, head);
     const Scores scores(p, head);
     const bool plain = scores.as_they_are();
@@ -939,11 +1023,11 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch
     TileLoads<S> next_q, next_g;
     RowLoads next = {};
     auto request = [&](int row0) {
-      next_q.request(queries, row0, p.nq, width_bytes, wave, lane);
-      next_g.request(grads, row0, p.nq, width_bytes, wave, lane);
+      next_q.request(queries, row0, last, width_bytes, wave, lane);
+      next_g.request(grads, row0, last, width_bytes, wave, lane);
       const int row = row0 + (int)threadIdx.x;
       if ((int)threadIdx.x < S::RT) {
-        const bool there = row < p.nq;
+        const bool there = row < last;
         const long long stat = ((long long)at.b * p.heads + head) * p.nq + row;
         next.segment = there ? (q_segments != nullptr ? q_segments[row] : 0) : kHiddenColumn;
         next.lse = there ? p.lse[stat] : kInf;
@@ -951,10 +1035,10 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch
         if (scores.apart) next.point = there ? reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + row] : f32x2{0.f, 0.f};
       }
     };
-    auto put = [&](char *tile, int, bool every) {
+    auto put = [&](char *tile, bool every) {
       if (!every)
 #pragma unroll
-        for (int u = 0; u < S::RT / 64; ++u) {
+        for (int u = 0; u < S::kCarried; ++u) {
           const bool bad_q = next_q.clear_bad(u), bad_g = next_g.clear_bad(u);
           put_poison<S>(tile, u, bad_q || bad_g, wave, lane);
         }
@@ -987,36 +1071,49 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch
           }
         }
         const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
-        if (!plain) finish_scores<S>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
+        finish_scores<Tag, true, 2, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
         const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
         const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
         const float *lse = reinterpret_cast<const float *>(tile + S::kLse) + block * 16 + 4 * g;
         const float *delta = reinterpret_cast<const float *>(tile + S::kDelta) + block * 16 + 4 * g;
+        if (!every)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[h][f][r] += poison[h * 16 + r];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int f = 0; f < S::CF; ++f) {
-              float x = s[h][f][r];
-              if (!every) x += poison[h * 16 + r];
-              float w = __builtin_amdgcn_exp2f(fmaf(x, factor, -lse[h * 16 + r]));
-              float dx = w * (t[h][f][r] - delta[h * 16 + r]);
-              if (scores.bent) dx *= bend[h][f][r];
-              if (!every) {
-                const bool seen = (uint32_t)(segments[h * 16 + r] - low[f]) <= span[f];
-                w = seen ? w : 0.f;
-                dx = seen ? dx : 0.f;
-              }
-              s[h][f][r] = w;
-              t[h][f][r] = dx;
+              s[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[h][f][r], factor, -lse[h * 16 + r]));
+              t[h][f][r] = s[h][f][r] * (t[h][f][r] - delta[h * 16 + r]);
             }
+        if (scores.bent)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int f = 0; f < S::CF; ++f) t[h][f] *= bend[h][f];
+        if (!every)      // whatever there is of a pair that is not seen
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int f = 0; f < S::CF; ++f) {
+                const bool seen = (uint32_t)(segments[h * 16 + r] - low[f]) <= span[f];
+                s[h][f][r] = seen ? s[h][f][r] : 0.f;
+                t[h][f][r] = seen ? t[h][f][r] : 0.f;
+              }
         add_product<S>(dv, tile + S::kTensorBytes, block, s, lane);
         up.apply(t, dk);
         add_product<S>(dk, tile, block, t, lane);
       }
     };
-    walk_tiles<S, true>(q_segments, masked, range, 0, p.nq, lds, s_flags, wave, lane, request, put, work);
+    walk_tiles<S, true>(q_segments, masked, range, first, last, lds, s_flags, wave, lane, request, put, work);
   }
 
   const float down = __builtin_amdgcn_exp2f(-kBackwardShift<Tag>);
@@ -1033,23 +1130,36 @@ __global__ void __launch_bounds__(kThreads) attn_grad_kv_kernel(const AttnLaunch
   for (int f = 0; f < S::CF; ++f) {
     const int j = mine0 + 16 * f + c;
     if (j >= p.nk) continue;
-    const size_t row = ((size_t)at.b * p.nk + j) * p.kv_heads + at.head;
+    const size_t rows = (size_t)p.batch * p.nk * p.kv_heads, row = ((size_t)at.b * p.nk + j) * p.kv_heads + at.head;
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) {
       if (!holds<S>(d, row_wave) || d * 16 + g * 4 >= p.width) continue;
-      if (p.grad_k != nullptr) store4<Tag>(p.grad_k, row * p.width + d * 16 + g * 4, dk[d][f]);
-      if (p.grad_v != nullptr) store4<Tag>(p.grad_v, row * p.width + d * 16 + g * 4, dv[d][f]);
+      store_grad<Tag>(p.grad_k, parts.part, 2 * at.chunk * rows, row, p.width, d * 16 + g * 4, dk[d][f]);
+      store_grad<Tag>(p.grad_v, parts.part, (2 * at.chunk + 1) * rows, row, p.width, d * 16 + g * 4, dv[d][f]);
     }
   }
 }
 
+// The chunks' parts, [chunk][tensors][elements], added in order and rounded: a lane takes four elements of one of the tensors.
+template <typename Tag>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_grads_kernel(const float *part, int chunks, long long elements, void *first, void *second) {
+  const int tensors = gridDim.y;
+  const long long at = ((long long)blockIdx.x * kJoinThreads + threadIdx.x) * 4;
+  void *to = blockIdx.y == 0 ? first : second;
+  if (at >= elements || to == nullptr) return;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int k = 0; k < chunks; ++k) sum += *reinterpret_cast<const f32x4 *>(part + ((long long)k * tensors + blockIdx.y) * elements + at);
+  store4<Tag>(to, at, sum);
+}
+
 // Sums of the slopes' parts of a head, [batch][heads][parts], in a fixed order.
-__global__ void __launch_bounds__(kThreads) attn_slope_grad_kernel(const float *part, float *grad, int batch, int heads, int parts) {
-  __shared__ float s_sum[kWaves];
+__global__ void __launch_bounds__(kJoinThreads) attn_slope_grad_kernel(const float *part, float *grad, int batch, int heads, int parts) {
+  __shared__ float s_sum[kJoinWaves];
   const int head = blockIdx.x, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   float sum = 0.f;
   for (int b = 0; b < batch; ++b)
-    for (int i = threadIdx.x; i < parts; i += kThreads) sum += part[((size_t)b * heads + head) * parts + i];
+    for (int i = threadIdx.x; i < parts; i += kJoinThreads) sum += part[((size_t)b * heads + head) * parts + i];
   sum = cluster_sum(sum, kWave);
   if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
@@ -1060,25 +1170,47 @@ __global__ void __launch_bounds__(kThreads) attn_slope_grad_kernel(const float *
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-enum Mode { kWide2, kWide1, kSplitRows };
-// Columns a workgroup: 128, 64, or 16 with the four waves dividing the rows.
-Mode column_mode(long long heads, int columns) {
-  if (heads * ceil_div(columns, 128) >= 512) return kWide2;
-  return heads * ceil_div(columns, 64) >= 256 ? kWide1 : kSplitRows;
+// Lanes that hold a row in fours, a power of two.
+int row_lanes(const AttnLaunch &p) {
+  int lanes = 2;
+  while (lanes * 4 < p.width) lanes *= 2;
+  return lanes;
 }
+
+// Columns a workgroup: many share the loads of a tile, few make workgroups for all CUs.  The most of which each CU gets one; with 16
+// the four waves divide the rows, as they do in part with 64 and 32.  us of the forward kernel with 128 / 64 / 32 / 16 columns, heads of 32, 16
+// bits: 8 heads x 300 queries 12.1 / 13.1 / 9.8 / 7.6; 16 x 1100 20.9 / 19.2 / 25.8 / 29.7; 32 x 1100 28.7 / 31.0 / 38.8 / 49.5; 32 x 2500
+// 82 / 85 / 113 / 165.  The gradients' kernels go the same way: dK and dV 16.8 / 11.4 / 9.9 / 7.9 and 33.9 / 28.6 / 34.7 / 42.0 for the first two.
+enum Mode { kColumns128, kColumns64, kColumns32, kColumns16 };
+Mode column_mode(long long heads, int columns) {
+  if (heads * ceil_div(columns, 128) >= 256) return kColumns128;
+  if (heads * ceil_div(columns, 64) >= 256) return kColumns64;
+  return heads * ceil_div(columns, 32) >= 256 ? kColumns32 : kColumns16;
+}
+// Rows of a tile and sixteens of columns a wave, by the bytes of a row: narrow rows make long tiles; a wave with two sixteens reads half as
+// much LDS, but backward it has no room for rows of 256 bytes (the gradients' kernels, 16 heads of 128, 4096 queries, 16 bits: 1560 us for 857).
 template <typename Tag, int W>
-struct Modes {
-  static constexpr bool kLarge = W * Tag::kBytes > 256;
-  typedef Shape<Tag, W, 64, 1, kLarge ? 1 : 2> Wide2;
-  typedef Shape<Tag, W, 64, 1, 1> Wide1;
-  typedef Shape<Tag, W, kLarge ? 64 : 128, kLarge ? 2 : 4, 1> SplitRows;
+struct ForwardModes {
+  static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 256 ? 1 : 2;
+  typedef Shape<Tag, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
+  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 256 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), (kBytes > 128 ? 1 : 2), 4> Columns32;
+  typedef Shape<Tag, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
+};
+template <typename Tag, int W>
+struct BackwardModes {
+  static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 128 ? 1 : 2;
+  typedef Shape<Tag, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
+  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), kTwo, 4> Columns32;
+  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
 };
 
 template <typename S, typename... A>
 hipError_t run(void (*kernel)(A...), long long blocks, hipStream_t stream, A... args) {
   if (S::kLdsBytes > (int)kMaxDynamicLds)
     if (hipError_t e = ensure_dynamic_lds_limit(reinterpret_cast<const void *>(kernel), S::kLdsBytes)) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), S::kLdsBytes, stream, args...);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(S::kThreads), S::kLdsBytes, stream, args...);
   return hipGetLastError();
 }
 
@@ -1103,7 +1235,7 @@ size_t part_bytes(const AttnLaunch &p, const Split &s) {
   return s.chunks > 1 ? padded((size_t)s.chunks * p.batch * p.nq * p.heads * p.width * sizeof(float)) : 0;
 }
 size_t forward_bytes(const AttnLaunch &p, const Split &s) {
-  return s.chunks > 1 ? part_bytes(p, s) + padded((size_t)s.chunks * p.batch * p.nq * p.heads * 2 * sizeof(float)) : 0;
+  return s.chunks > 1 ? part_bytes(p, s) + padded((size_t)s.chunks * p.batch * p.nq * p.heads * 4 * sizeof(float)) : 0;
 }
 
 template <typename S>
@@ -1119,46 +1251,120 @@ hipError_t forward_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
   const long long blocks = (long long)p.batch * p.heads * s.tiles * s.chunks;
   if (hipError_t e = run<S>(attn_forward_kernel<S>, blocks, stream, p, s)) return e;
   if (s.chunks == 1) return hipSuccess;
-  const long long lanes = (long long)p.batch * p.nq * p.heads * (p.width / 4);
-  hipLaunchKernelGGL((attn_join_kernel<Tag>), dim3((unsigned)ceil_div(lanes, kThreads)), dim3(kThreads), 0, stream, p, s);
+  hipLaunchKernelGGL((attn_join_kernel<Tag>), dim3((unsigned)ceil_div((long long)p.batch * p.nq * p.heads, kJoinWaves)), dim3(kJoinThreads), 0, stream, p, s,
+                     row_lanes(p));
   return hipGetLastError();
 }
 
+// Chunks of the rows, where the columns' workgroups leave much of the chip free; each has some tiles of work.
 template <typename S>
-hipError_t grad_q_shape(const AttnLaunch &p, BackwardParts parts, hipStream_t stream) {
+void divide_rows(BackwardParts *parts, long long blocks, int rows, int head_parts) {
+  const int row_tiles = std::max(1, ceil_div(rows, S::RT));
+  int per_chunk = row_tiles;
+  if (blocks * head_parts < 192) per_chunk = ceil_div(row_tiles, std::max(1, (int)std::min<long long>(512 / (blocks * head_parts), row_tiles / 4)));
+  parts->chunk_rows = per_chunk * S::RT;
+  parts->head_parts = head_parts;
+  parts->chunks = ceil_div(row_tiles, per_chunk) * head_parts;
+}
+template <typename S>
+BackwardParts plan_grad_q(const AttnLaunch &p) {
+  BackwardParts parts = {};
   parts.tiles = ceil_div(p.nq, S::kColumns);
-  if (hipError_t e = run<S>(attn_grad_q_kernel<S>, (long long)p.batch * p.heads * parts.tiles, stream, p, parts)) return e;
-  if (parts.slopes == nullptr) return hipSuccess;
-  hipLaunchKernelGGL(attn_slope_grad_kernel, dim3(p.heads), dim3(kThreads), 0, stream, parts.slopes, p.grad_slopes, p.batch, p.heads, parts.tiles);
+  const long long blocks = (long long)p.batch * p.heads * parts.tiles;
+  // (the slopes' sums are of whole rows)
+  divide_rows<S>(&parts, p.slopes != nullptr ? 512 : blocks, p.nk, 1);
+  return parts;
+}
+template <typename S>
+BackwardParts plan_grad_kv(const AttnLaunch &p) {
+  BackwardParts parts = {};
+  parts.tiles = ceil_div(p.nk, S::kColumns);
+  const long long blocks = (long long)p.batch * p.kv_heads * parts.tiles;
+  divide_rows<S>(&parts, blocks, p.nq, blocks < 2048 ? p.heads / p.kv_heads : 1);
+  return parts;
+}
+size_t delta_bytes(const AttnLaunch &p) { return padded((size_t)p.batch * p.heads * p.nq * sizeof(float)); }
+size_t slope_bytes(const AttnLaunch &p) {      // of 16 columns or more each
+  return p.slopes != nullptr ? padded((size_t)p.batch * p.heads * ceil_div(p.nq, 16) * sizeof(float)) : 0;
+}
+size_t query_elements(const AttnLaunch &p) { return (size_t)p.batch * p.nq * p.heads * p.width; }
+size_t key_elements(const AttnLaunch &p) { return (size_t)p.batch * p.nk * p.kv_heads * p.width; }
+
+// delta, the slopes' parts, then the chunks of the kernel at work
+template <typename S>
+hipError_t grad_q_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  typedef typename S::Tag Tag;
+  BackwardParts parts = plan_grad_q<S>(p);
+  if (bytes != nullptr) {
+    *bytes = parts.chunks > 1 ? padded(parts.chunks * query_elements(p) * sizeof(float)) : 0;
+    return hipSuccess;
+  }
+  char *ws = static_cast<char *>(p.workspace);
+  parts.delta = reinterpret_cast<float *>(ws);
+  if (p.grad_slopes != nullptr) parts.slopes = reinterpret_cast<float *>(ws + delta_bytes(p));
+  if (parts.chunks > 1) parts.part = reinterpret_cast<float *>(ws + delta_bytes(p) + slope_bytes(p));
+  if (hipError_t e = run<S>(attn_grad_q_kernel<S>, (long long)p.batch * p.heads * parts.tiles * parts.chunks, stream, p, parts)) return e;
+  if (parts.slopes != nullptr) {
+    hipLaunchKernelGGL(attn_slope_grad_kernel, dim3(p.heads), dim3(kJoinThreads), 0, stream, parts.slopes, p.grad_slopes, p.batch, p.heads, parts.tiles);
+    if (hipError_t e = hipGetLastError()) return e;
+  }
+  if (parts.chunks == 1 || p.grad_q == nullptr) return hipSuccess;
+  const long long n = (long long)query_elements(p);
+  hipLaunchKernelGGL((attn_join_grads_kernel<Tag>), dim3(ceil_div(n, 4 * kJoinThreads)), dim3(kJoinThreads), 0, stream, parts.part, parts.chunks, n, p.grad_q,
+                     (void *)nullptr);
   return hipGetLastError();
 }
 template <typename S>
-hipError_t grad_kv_shape(const AttnLaunch &p, BackwardParts parts, hipStream_t stream) {
-  parts.tiles = ceil_div(p.nk, S::kColumns);
-  return run<S>(attn_grad_kv_kernel<S>, (long long)p.batch * p.kv_heads * parts.tiles, stream, p, parts);
+hipError_t grad_kv_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  typedef typename S::Tag Tag;
+  BackwardParts parts = plan_grad_kv<S>(p);
+  if (bytes != nullptr) {
+    *bytes = parts.chunks > 1 ? padded(2 * parts.chunks * key_elements(p) * sizeof(float)) : 0;
+    return hipSuccess;
+  }
+  char *ws = static_cast<char *>(p.workspace);
+  parts.delta = reinterpret_cast<float *>(ws);
+  if (parts.chunks > 1) parts.part = reinterpret_cast<float *>(ws + delta_bytes(p) + slope_bytes(p));
+  if (hipError_t e = run<S>(attn_grad_kv_kernel<S>, (long long)p.batch * p.kv_heads * parts.tiles * parts.chunks, stream, p, parts)) return e;
+  if (parts.chunks == 1) return hipSuccess;
+  const long long n = (long long)key_elements(p);
+  hipLaunchKernelGGL((attn_join_grads_kernel<Tag>), dim3(ceil_div(n, 4 * kJoinThreads), 2), dim3(kJoinThreads), 0, stream, parts.part, parts.chunks, n, p.grad_k,
+                     p.grad_v);
+  return hipGetLastError();
 }
 
 template <typename Tag, int W>
 hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  typedef Modes<Tag, W> M;
+  typedef ForwardModes<Tag, W> M;
   switch (column_mode((long long)p.batch * p.heads, p.nq)) {
-    case kWide2: return forward_shape<typename M::Wide2>(p, stream, bytes);
-    case kWide1: return forward_shape<typename M::Wide1>(p, stream, bytes);
-    default: return forward_shape<typename M::SplitRows>(p, stream, bytes);
+    case kColumns128: return forward_shape<typename M::Columns128>(p, stream, bytes);
+    case kColumns64: return forward_shape<typename M::Columns64>(p, stream, bytes);
+    case kColumns32: return forward_shape<typename M::Columns32>(p, stream, bytes);
+    default: return forward_shape<typename M::Columns16>(p, stream, bytes);
   }
 }
-size_t delta_bytes(const AttnLaunch &p) { return padded((size_t)p.batch * p.heads * p.nq * sizeof(float)); }
 
 template <typename Tag, int W>
-hipError_t backward_width(const AttnLaunch &p, hipStream_t stream) {
-  typedef Modes<Tag, W> M;
-  BackwardParts parts = {static_cast<float *>(p.workspace), nullptr, 0};
-  if (p.grad_slopes != nullptr) parts.slopes = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + delta_bytes(p));
-  hipError_t e = column_mode((long long)p.batch * p.heads, p.nq) == kSplitRows ? grad_q_shape<typename M::SplitRows>(p, parts, stream)
-                                                                               : grad_q_shape<typename M::Wide1>(p, parts, stream);
-  if (e != hipSuccess || (p.grad_k == nullptr && p.grad_v == nullptr)) return e;
-  return column_mode((long long)p.batch * p.kv_heads, p.nk) == kSplitRows ? grad_kv_shape<typename M::SplitRows>(p, parts, stream)
-                                                                          : grad_kv_shape<typename M::Wide1>(p, parts, stream);
+hipError_t backward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  typedef BackwardModes<Tag, W> M;
+  const bool keys = bytes != nullptr || p.grad_k != nullptr || p.grad_v != nullptr;
+  size_t q_bytes = 0, kv_bytes = 0;
+  hipError_t e = hipSuccess;
+  switch (column_mode((long long)p.batch * p.heads, p.nq)) {
+    case kColumns128: e = grad_q_shape<typename M::Columns128>(p, stream, bytes ? &q_bytes : nullptr); break;
+    case kColumns64: e = grad_q_shape<typename M::Columns64>(p, stream, bytes ? &q_bytes : nullptr); break;
+    case kColumns32: e = grad_q_shape<typename M::Columns32>(p, stream, bytes ? &q_bytes : nullptr); break;
+    default: e = grad_q_shape<typename M::Columns16>(p, stream, bytes ? &q_bytes : nullptr);
+  }
+  if (e != hipSuccess || !keys) return e;
+  switch (column_mode((long long)p.batch * p.kv_heads, p.nk)) {
+    case kColumns128: e = grad_kv_shape<typename M::Columns128>(p, stream, bytes ? &kv_bytes : nullptr); break;
+    case kColumns64: e = grad_kv_shape<typename M::Columns64>(p, stream, bytes ? &kv_bytes : nullptr); break;
+    case kColumns32: e = grad_kv_shape<typename M::Columns32>(p, stream, bytes ? &kv_bytes : nullptr); break;
+    default: e = grad_kv_shape<typename M::Columns16>(p, stream, bytes ? &kv_bytes : nullptr);
+  }
+  if (bytes != nullptr) *bytes = delta_bytes(p) + slope_bytes(p) + std::max(q_bytes, kv_bytes);
+  return e;
 }
 
 template <typename Tag>
@@ -1167,9 +1373,17 @@ hipError_t forward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
   return p.width <= 64 ? forward_width<Tag, 64>(p, stream, bytes) : forward_width<Tag, 128>(p, stream, bytes);
 }
 template <typename Tag>
-hipError_t backward_t(const AttnLaunch &p, hipStream_t stream) {
-  if (p.width <= 32) return backward_width<Tag, 32>(p, stream);
-  return p.width <= 64 ? backward_width<Tag, 64>(p, stream) : backward_width<Tag, 128>(p, stream);
+hipError_t backward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  if (p.width <= 32) return backward_width<Tag, 32>(p, stream, bytes);
+  return p.width <= 64 ? backward_width<Tag, 64>(p, stream, bytes) : backward_width<Tag, 128>(p, stream, bytes);
+}
+hipError_t backward(int dtype, const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  switch (dtype) {
+    case F32::kCode: return backward_t<F32>(p, stream, bytes);
+    case F16::kCode: return backward_t<F16>(p, stream, bytes);
+    case BF16::kCode: return backward_t<BF16>(p, stream, bytes);
+  }
+  return hipErrorInvalidValue;
 }
 hipError_t forward(int dtype, const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
   switch (dtype) {
@@ -1187,19 +1401,13 @@ size_t attn_forward_workspace_bytes(int dtype, const AttnLaunch &p) {
   if (forward(dtype, p, nullptr, &bytes) != hipSuccess) return 0;      // the launch says why
   return bytes;
 }
-size_t attn_backward_workspace_bytes(int, const AttnLaunch &p) {
-  // a part of the slopes' gradient for 16 columns or more
-  return delta_bytes(p) + (p.slopes != nullptr ? padded((size_t)p.batch * p.heads * ceil_div(p.nq, 16) * sizeof(float)) : 0);
+size_t attn_backward_workspace_bytes(int dtype, const AttnLaunch &p) {
+  size_t bytes = 0;
+  if (backward(dtype, p, nullptr, &bytes) != hipSuccess) return 0;
+  return bytes;
 }
 
 hipError_t launch_attn_forward(int dtype, const AttnLaunch &p, hipStream_t stream) { return forward(dtype, p, stream, nullptr); }
-hipError_t launch_attn_backward(int dtype, const AttnLaunch &p, hipStream_t stream) {
-  switch (dtype) {
-    case F32::kCode: return backward_t<F32>(p, stream);
-    case F16::kCode: return backward_t<F16>(p, stream);
-    case BF16::kCode: return backward_t<BF16>(p, stream);
-  }
-  return hipErrorInvalidValue;
-}
+hipError_t launch_attn_backward(int dtype, const AttnLaunch &p, hipStream_t stream) { return backward(dtype, p, stream, nullptr); }
 
 }  // namespace dcn

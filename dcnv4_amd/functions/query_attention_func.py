@@ -63,7 +63,7 @@ def query_attention(query, key, value, *, scale=None, cap=0.0, segments=None, ke
         if points is not None and points.requires_grad:
             raise RuntimeError("query_attention has no gradient for positions: detach them")
     if torch.is_autocast_enabled() and query.is_cuda:
-        dtype = torch.get_autocast_gpu_dtype()
+        dtype = torch.get_autocast_dtype("cuda")
         query, key, value = (t.to(dtype) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (query, key, value))
     if key_segments is None:
         key_segments = segments
