@@ -76,7 +76,8 @@ struct Shape {
 // ---------------------------------------------------------------- a tile's way into LDS
 // Rows in slices of 64 bytes, 16 to a block of 1 KB, a row's vectors at vector ^ (row / 4 & 3) (fragment_offset): both the fragment
 // reads and the transposing ones then spread over the banks.  A wave carries sixteens of rows, four lanes a row.
-__device__ __forceinline__ uint32_t fragment_at(int r16, int kb) { return (uint32_t)(r16 * 64 + (kb ^ ((r16 >> 2) & 3)) * 16); }
+__device__ __forceinline__ int turned_by(int r4) { return -r4 & 3; }      // of rows 4 r4 .. + 3 of sixteen
+__device__ __forceinline__ uint32_t fragment_at(int r16, int kb) { return (uint32_t)(r16 * 64 + (kb ^ turned_by(r16 >> 2)) * 16); }
 
 struct HeadRows {
   const char *base;
@@ -93,7 +94,7 @@ struct TileLoads {
 
   __device__ __forceinline__ void request(const HeadRows &t, int row0, int rows, int width_bytes, int wave, int lane) {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(t.base + row0 * t.pitch, 0x7fffffffu);
-    const int vec = (lane & 3) ^ ((lane >> 4) & 3);
+    const int vec = (lane & 3) ^ turned_by(lane >> 4);
 #pragma unroll
     for (int u = 0; u < S::kCarried; ++u) {
       const int row = (wave + S::kWaves * u) * 16 + lane / 4;
@@ -155,7 +156,7 @@ __device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF]
     }
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) {
-      const char *at = tensor + d / 2 * S::RT * 64 + block * 1024 + (4 * g + (c >> 2)) * 64 + (((d & 1) * 2 + ((c & 3) >> 1)) ^ g) * 16 + (c & 1) * 8;
+      const char *at = tensor + d / 2 * S::RT * 64 + block * 1024 + (4 * g + (c >> 2)) * 64 + (((d & 1) * 2 + ((c & 3) >> 1)) ^ turned_by(g)) * 16 + (c & 1) * 8;
       typedef __attribute__((address_space(3))) s16x4 lds_words;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_words *)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_words *)(at + 1024));
       const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
@@ -168,7 +169,7 @@ __device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF]
     for (int d = 0; d < S::kWidthBlocks; ++d)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const char *at = tensor + d * S::RT * 64 + (block + half) * 1024 + 4 * g * 64 + ((c >> 2) ^ g) * 16 + (c & 3) * 4;
+        const char *at = tensor + d * S::RT * 64 + (block + half) * 1024 + 4 * g * 64 + ((c >> 2) ^ turned_by(g)) * 16 + (c & 3) * 4;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float a = *reinterpret_cast<const float *>(at + r * 64);
@@ -217,30 +218,40 @@ struct Scores {
   }
   __device__ __forceinline__ bool as_they_are() const { return !bent && !scaled; }
 };
+// tanh(x) = 1 - 2 r with r = 1 / (exp(2 x) + 1), whose derivative is 4 (r - r^2): 16-bit types carry r - r^2 and the factor at the end.
+template <typename Tag> constexpr float kBendFactor = Tag::kBytes == 4 ? 1.f : 4.f;
 __device__ __forceinline__ float distance(f32x2 a, f32x2 b) {
   const float x = a.x - b.x, y = a.y - b.y;
   return __builtin_amdgcn_sqrtf(fmaf(x, x, y * y));
 }
 
-// Scores of N blocks of 16 rows, from the products in s; point_of(n, r): the rows' positions.  With GRADS also the distances and
-// 1 - tanh^2.  What a call has is the same for all lanes: a loop for each, not a question for each score.
-template <typename Tag, bool GRADS, int N, int CF, typename Points>
-__device__ __forceinline__ void finish_scores(const Scores &scores, f32x4 (&s)[N][CF], f32x4 (&far)[GRADS ? N : 1][CF], f32x4 (&bend)[GRADS ? N : 1][CF],
-                                              const f32x2 (&point)[CF], Points point_of) {
+// Scores of N blocks of 16 rows, from the products in s.  What a call has is the same for all lanes: a loop for each, not a question
+// for each score.  Forward; `point` and what point_of(n, r) gives, the rows' positions, come multiplied by the slope where `stretched`
+// says so.
+template <typename Tag, int N, int CF, typename Points>
+__device__ __forceinline__ void finish_scores(const Scores &scores, bool stretched, f32x4 (&s)[N][CF], const f32x2 (&point)[CF], Points point_of) {
   if (scores.bent) {
-    const float rate = scores.tanh_scale * (2.f * kLog2e);
+    const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int f = 0; f < CF; ++f)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float t;
-          if constexpr (Tag::kBytes == 4) t = tanhf(s[n][f][r] * scores.tanh_scale);      // fp32 results see the last bits
-          else t = fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][f][r] * rate) + 1.f), 1.f);
-          if constexpr (GRADS) bend[n][f][r] = fmaf(-t, t, 1.f);
-          s[n][f][r] = t * scores.factor;
+          if constexpr (Tag::kBytes == 4) s[n][f][r] = tanhf(s[n][f][r] * scores.tanh_scale) * scores.factor;      // fp32 results see the last bits
+          else s[n][f][r] = fmaf(twice, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][f][r] * rate) + 1.f), scores.factor);
         }
+  }
+  if (stretched) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x2 there = point_of(n, r);
+#pragma unroll
+        for (int f = 0; f < CF; ++f) s[n][f][r] = fmaf(s[n][f][r], scores.factor, -distance(point[f], there));
+      }
+    return;
   }
   if (scores.scaled)
 #pragma unroll
@@ -254,12 +265,69 @@ __device__ __forceinline__ void finish_scores(const Scores &scores, f32x4 (&s)[N
       for (int r = 0; r < 4; ++r) {
         const f32x2 there = point_of(n, r);
 #pragma unroll
+        for (int f = 0; f < CF; ++f) s[n][f][r] = fmaf(-scores.slope, distance(point[f], there), s[n][f][r]);
+      }
+}
+// Backward: weights of 32 rows without what is not seen, from the products in s and the rows' or columns' logarithms; the distances,
+// and the tanh's derivative over kBendFactor.  seen(): masks s in place, before the exponential.
+template <typename Tag, int CF, typename Points, typename Lse, typename Seen>
+__device__ __forceinline__ void form_weights(const Scores &scores, f32x4 (&s)[2][CF], f32x4 (&far)[2][CF], f32x4 (&bend)[2][CF], const f32x2 (&point)[CF],
+                                             Points point_of, Lse lse, Seen seen) {
+  if (scores.as_they_are()) {
+    seen();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int f = 0; f < CF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[h][f][r], scores.factor, -lse(h, r, f)));
+    return;
+  }
+  if (scores.bent) {
+    const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int f = 0; f < CF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (Tag::kBytes == 4) {
+            const float t = tanhf(s[h][f][r] * scores.tanh_scale);
+            bend[h][f][r] = fmaf(-t, t, 1.f);
+            s[h][f][r] = fmaf(t, scores.factor, -lse(h, r, f));
+          } else {
+            const float t = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[h][f][r] * rate) + 1.f);
+            bend[h][f][r] = fmaf(-t, t, t);
+            s[h][f][r] = fmaf(twice, t, scores.factor - lse(h, r, f));
+          }
+        }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int f = 0; f < CF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[h][f][r] = fmaf(s[h][f][r], scores.factor, -lse(h, r, f));
+  }
+  if (scores.apart)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x2 there = point_of(h, r);
+#pragma unroll
         for (int f = 0; f < CF; ++f) {
-          const float d = distance(point[f], there);
-          if constexpr (GRADS) far[n][f][r] = d;
-          s[n][f][r] = fmaf(-scores.slope, d, s[n][f][r]);
+          far[h][f][r] = distance(point[f], there);
+          s[h][f][r] = fmaf(-scores.slope, far[h][f][r], s[h][f][r]);
         }
       }
+  seen();
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int f = 0; f < CF; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[h][f][r] = __builtin_amdgcn_exp2f(s[h][f][r]);
 }
 
 // ---------------------------------------------------------------- which tiles
@@ -455,6 +523,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
   const Scores scores(p, at.head);
   const bool plain = scores.as_they_are(), masked = p.k_segments != nullptr;
   const float factor = plain ? scores.factor : 1.f;
+  // without a cap the product's factor and the distance are one operation, if the positions carry the slope
+  const bool stretched = scores.apart && !scores.bent && scores.slope >= 0.f;
+  const float stretch = stretched ? scores.slope : 1.f;
 
   u32x4 q[S::CF][S::kSlices];
   load_columns<S>(q, head_rows<Tag>(p.q, at.b, at.head), mine0, p.nq, width_bytes, lane);
@@ -468,7 +539,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
     segment[f] = i < p.nq ? (q_segments != nullptr ? q_segments[i] : 0) : kHiddenColumn;
     if (segment[f] < 0) segment[f] = kHiddenColumn;
     point[f] = f32x2{0.f, 0.f};
-    if (scores.apart && i < p.nq) point[f] = reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + i];
+    if (scores.apart && i < p.nq) point[f] = reinterpret_cast<const f32x2 *>(p.q_points)[(long long)at.b * p.nq + i] * stretch;
   }
   const ColumnRange range = masked ? column_range<false>(q_segments, column0, p.nq, S::kColumns, lane) : ColumnRange{};
 
@@ -505,7 +576,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
     next_v.put(tile + S::kTensorBytes, wave, lane);
     if ((int)threadIdx.x < S::RT) {
       reinterpret_cast<int *>(tile + S::kSegments)[threadIdx.x] = next.segment;
-      if (scores.apart) reinterpret_cast<f32x2 *>(tile + S::kPoints)[threadIdx.x] = next.point;
+      if (scores.apart) reinterpret_cast<f32x2 *>(tile + S::kPoints)[threadIdx.x] = next.point * stretch;
     }
   };
   auto work = [&](const char *tile, bool every) {
@@ -523,8 +594,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
       }
     }
     const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block0 * 16 + 4 * g;
-    f32x4 unused[1][S::CF];
-    finish_scores<Tag, false, S::kRowBlocks, S::CF>(scores, s, unused, unused, point, [&](int n, int r) { return points[n * 16 + r]; });
+    finish_scores<Tag, S::kRowBlocks, S::CF>(scores, stretched, s, point, [&](int n, int r) { return points[n * 16 + r]; });
     if (!every)
 #pragma unroll
       for (int n = 0; n < S::kRowBlocks; ++n) {
@@ -768,8 +838,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
   const int first = at.chunk * parts.chunk_rows, last = min(p.nk, first + parts.chunk_rows);
   const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
   const Scores scores(p, at.head);
-  const bool plain = scores.as_they_are(), masked = p.k_segments != nullptr;
-  const float factor = plain ? scores.factor : 1.f;
+  const bool masked = p.k_segments != nullptr;
 
   u32x4 q[S::CF][S::kSlices], go[S::CF][S::kSlices];
   load_columns<S>(q, head_rows<Tag>(p.q, at.b, at.head), mine0, p.nq, width_bytes, lane);
@@ -819,12 +888,16 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
     for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   ColumnScale<S> up;
   // The slopes' gradient is fp32 and a sum of terms that nearly cancel in each row: delta, which is as exact as the forward's weights
-  // were rounded, would show.  With w the weights formed here, a row adds -sum w (t - mean) distance, mean = sum w t / sum w: four
-  // sums a column, over w (t - delta) = dS for t to keep them small.  Sums of w, w distance, dS, dS distance:
+  // were rounded, would show.  A row adds -sum dS distance with dS = w (t - delta), less delta's error sum dS times sum w distance
+  // (the weights add up to 1): sums of dS, w distance, dS distance.
   const bool want_slopes = parts.slopes != nullptr;
-  f32x4 moment[S::CF];
+  float moment[S::CF][3];
+  f32x4 minus_delta[S::CF];      // what the product dO V^T starts from
 #pragma unroll
-  for (int f = 0; f < S::CF; ++f) moment[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int f = 0; f < S::CF; ++f) {
+    moment[f][0] = moment[f][1] = moment[f][2] = 0.f;
+    minus_delta[f] = f32x4{-delta[f], -delta[f], -delta[f], -delta[f]};
+  }
 
   TileLoads<S> next_k, next_v;
   RowLoads next = {};
@@ -856,7 +929,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int f = 0; f < S::CF; ++f) s[h][f] = t[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < S::CF; ++f) {
+          s[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+          t[h][f] = minus_delta[f];
+        }
 #pragma unroll
         for (int sl = 0; sl < S::kSlices; ++sl) {
           const u32x4 a = fragment<S>(tile, block + h, sl, lane), b = fragment<S>(tile + S::kTensorBytes, block + h, sl, lane);
@@ -868,10 +944,10 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
         }
       }
       const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
-      finish_scores<Tag, true, 2, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
       const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
       const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
-      if (!every)
+      form_weights<Tag, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int, int, int f) { return lse[f]; }, [&] {
+        if (every) return;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -881,19 +957,15 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
               const bool seen = segments[h * 16 + r] == 0 || segments[h * 16 + r] == segment[f];
               s[h][f][r] = seen ? s[h][f][r] + poison[h * 16 + r] : -kInf;
               // what else there is of a pair that is not seen may be anything
-              t[h][f][r] = seen ? t[h][f][r] : delta[f];
+              t[h][f][r] = seen ? t[h][f][r] : 0.f;
               if (scores.apart) far[h][f][r] = seen ? far[h][f][r] : 0.f;
               if (scores.bent) bend[h][f][r] = seen ? bend[h][f][r] : 0.f;
             }
+      });
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int f = 0; f < S::CF; ++f) {
-            s[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[h][f][r], factor, -lse[f]));
-            t[h][f][r] = s[h][f][r] * (t[h][f][r] - delta[f]);
-          }
+        for (int f = 0; f < S::CF; ++f) t[h][f] *= s[h][f];
       if (want_slopes)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -901,10 +973,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
           for (int f = 0; f < S::CF; ++f)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              moment[f].x += s[h][f][r];
-              moment[f].y = fmaf(s[h][f][r], far[h][f][r], moment[f].y);
-              moment[f].z += t[h][f][r];
-              moment[f].w = fmaf(t[h][f][r], far[h][f][r], moment[f].w);
+              moment[f][0] += t[h][f][r];
+              moment[f][1] = fmaf(s[h][f][r], far[h][f][r], moment[f][1]);
+              moment[f][2] = fmaf(t[h][f][r], far[h][f][r], moment[f][2]);
             }
       if (scores.bent)
 #pragma unroll
@@ -919,11 +990,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
 
 #pragma unroll
   for (int f = 0; f < S::CF; ++f) {
-    const float by = p.scale / up.by[f];
+    const float by = p.scale * (scores.bent ? kBendFactor<Tag> : 1.f) / up.by[f];
     const bool sees = segment[f] >= 0;
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = sees ? acc[d][f] * by : f32x4{0.f, 0.f, 0.f, 0.f};
-    if (!sees) moment[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!sees) moment[f][0] = moment[f][1] = moment[f][2] = 0.f;
   }
   merge_rows<S>(acc, lds, row_wave, column_wave, lane);
   const size_t rows_before = (size_t)at.chunk * p.batch * p.nq * p.heads;
@@ -942,26 +1013,26 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
 #pragma unroll
     for (int f = 0; f < S::CF; ++f)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) moment[f][e] = column_sum(moment[f][e]);
+      for (int e = 0; e < 3; ++e) moment[f][e] = column_sum(moment[f][e]);
     if constexpr (S::RW > 1) {
       f32x4 *s_stats = reinterpret_cast<f32x4 *>(lds + S::kMergeStats);
       auto slot = [&](int w, int f) { return ((w * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c; };
 #pragma unroll
       for (int f = 0; f < S::CF; ++f)
-        if (g == 0) s_stats[slot(row_wave, f)] = moment[f];
+        if (g == 0) s_stats[slot(row_wave, f)] = f32x4{moment[f][0], moment[f][1], moment[f][2], 0.f};
       __syncthreads();
 #pragma unroll
       for (int f = 0; f < S::CF; ++f) {
-        moment[f] = s_stats[slot(0, f)];
+        f32x4 all = s_stats[slot(0, f)];
 #pragma unroll
-        for (int w = 1; w < S::RW; ++w) moment[f] += s_stats[slot(w, f)];
+        for (int w = 1; w < S::RW; ++w) all += s_stats[slot(w, f)];
+        moment[f][0] = all.x; moment[f][1] = all.y; moment[f][2] = all.z;
       }
     }
     float sum = 0.f;
 #pragma unroll
     for (int f = 0; f < S::CF; ++f)
-      if (g == 0 && row_wave == 0 && mine0 + 16 * f + c < p.nq && moment[f].x != 0.f)
-        sum -= (moment[f].w - moment[f].z / moment[f].x * moment[f].y) / moment[f].x;
+      if (g == 0 && row_wave == 0 && mine0 + 16 * f + c < p.nq) sum -= moment[f][2] - moment[f][0] * moment[f][1];
     sum = cluster_sum(sum, kWave);
     if (lane == 0) s_slopes[wave] = sum;
     __syncthreads();
@@ -1018,8 +1089,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
   for (int head = head0; head < head0 + heads_here; ++head) {
     const HeadRows queries = head_rows<Tag>(p.q, at.b, head), grads = head_rows<Tag>(p.grad_out, at.b, head);
     const Scores scores(p, head);
-    const bool plain = scores.as_they_are();
-    const float factor = plain ? scores.factor : 1.f;
     TileLoads<S> next_q, next_g;
     RowLoads next = {};
     auto request = [&](int row0) {
@@ -1047,7 +1116,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
       if ((int)threadIdx.x < S::RT) {
         reinterpret_cast<int *>(tile + S::kSegments)[threadIdx.x] = max(next.segment, kHiddenColumn) == -1 ? kHiddenColumn : max(next.segment, kHiddenColumn);
         reinterpret_cast<float *>(tile + S::kLse)[threadIdx.x] = next.lse - kBackwardShift<Tag>;
-        reinterpret_cast<float *>(tile + S::kDelta)[threadIdx.x] = next.delta;
+        reinterpret_cast<float *>(tile + S::kDelta)[threadIdx.x] = -next.delta;      // what the product dO V^T starts from
         if (scores.apart) reinterpret_cast<f32x2 *>(tile + S::kPoints)[threadIdx.x] = next.point;
       }
     };
@@ -1056,10 +1125,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
       for (int n = 0; n < S::kRowBlocks; n += 2) {
         const int block = row_wave * S::kRowBlocks + n;
         f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
+        const f32x4 *minus_delta = reinterpret_cast<const f32x4 *>(tile + S::kDelta) + block * 4 + g;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int f = 0; f < S::CF; ++f) s[h][f] = t[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int f = 0; f < S::CF; ++f) {
+            s[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+            t[h][f] = minus_delta[h * 4];
+          }
 #pragma unroll
           for (int sl = 0; sl < S::kSlices; ++sl) {
             const u32x4 a = fragment<S>(tile, block + h, sl, lane), b = fragment<S>(tile + S::kTensorBytes, block + h, sl, lane);
@@ -1071,32 +1144,26 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
           }
         }
         const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
-        finish_scores<Tag, true, 2, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; });
         const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
         const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
         const float *lse = reinterpret_cast<const float *>(tile + S::kLse) + block * 16 + 4 * g;
-        const float *delta = reinterpret_cast<const float *>(tile + S::kDelta) + block * 16 + 4 * g;
-        if (!every)
+        form_weights<Tag, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int h, int r, int) { return lse[h * 16 + r]; },
+                                 [&] {
+                                   if (every) return;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+                                   for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int f = 0; f < S::CF; ++f)
+                                     for (int f = 0; f < S::CF; ++f)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) s[h][f][r] += poison[h * 16 + r];
+                                       for (int r = 0; r < 4; ++r) s[h][f][r] += poison[h * 16 + r];
+                                 });
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int f = 0; f < S::CF; ++f) {
-              s[h][f][r] = __builtin_amdgcn_exp2f(fmaf(s[h][f][r], factor, -lse[h * 16 + r]));
-              t[h][f][r] = s[h][f][r] * (t[h][f][r] - delta[h * 16 + r]);
-            }
-        if (scores.bent)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int f = 0; f < S::CF; ++f) t[h][f] *= bend[h][f];
+          for (int f = 0; f < S::CF; ++f) {
+            t[h][f] *= s[h][f];
+            if (scores.bent) t[h][f] *= bend[h][f];
+          }
         if (!every)      // whatever there is of a pair that is not seen
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -1121,7 +1188,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
   for (int f = 0; f < S::CF; ++f)
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) {
-      dk[d][f] *= p.scale * down / up.by[f];
+      dk[d][f] *= p.scale * (p.cap > 0.f ? kBendFactor<Tag> : 1.f) * down / up.by[f];
       dv[d][f] *= down;
     }
   merge_rows<S>(dk, lds, row_wave, column_wave, lane);
