@@ -3,8 +3,8 @@
 // xhat = (z - mean) * rstd and a = grad_out * weight,
 //   dz = rstd (a - mean(a) - xhat mean(a xhat)) + grad_sum,   dweight = sum over rows of grad_out xhat,   dbias = sum of grad_out
 //
-// HBM-bound: each tensor is read or written once.  A team of lanes (a power of two, up to a whole workgroup of 1024) owns a row, a
-// lane eight consecutive elements of it, which stay in registers as fp32 from the sum to the result: the sum is not rounded
+// HBM-bound: each tensor is read or written once.  A team of lanes (a power of two, up to a whole workgroup of 512) owns a row, a
+// lane eight or twice eight elements of it, which stay in registers as fp32 from the sum to the result: the sum is not rounded
 // before it is normalised.  The mean and the deviations about it are two reductions over the team; both are kept for the
 // backward, 8 bytes a row, which then reduces once.  A workgroup walks a slab of rows with the parameters in registers and the next
 // row's loads under way.  A row may start at any element and have any width: the loads are unaligned ones, the last
@@ -15,6 +15,7 @@
 #include "add_norm.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -75,36 +76,31 @@ __device__ __forceinline__ void store_vec(char *at, int live, const float (&f)[k
       reinterpret_cast<typename RawWord<Tag::kBytes>::type *>(at)[c] = Pack<Tag, 1>::encode(one);
     }
 }
-// The same by a type's code, one for all lanes.
+// Parameters go by their type's code, one for all lanes.
 __device__ __forceinline__ int bytes_of(int dtype) { return dtype == F32::kCode ? 4 : 2; }
-__device__ __forceinline__ void load_any(int dtype, const char *at, int live, Raw &r) {
-  if (dtype == F32::kCode) load_vec<F32>(at, live, r);
-  else load_vec<F16>(at, live, r);
-}
-__device__ __forceinline__ void decode_any(int dtype, const Raw &r, float (&f)[kVec]) {
-  if (dtype == F32::kCode) decode_vec<F32>(r, f);
-  else if (dtype == F16::kCode) decode_vec<F16>(r, f);
-  else decode_vec<BF16>(r, f);
-}
-__device__ __forceinline__ void store_any(int dtype, void *base, long long element, int live, const float (&f)[kVec]) {
-  char *at = static_cast<char *>(base) + element * bytes_of(dtype);
-  if (dtype == F32::kCode) store_vec<F32>(at, live, f);
-  else if (dtype == F16::kCode) store_vec<F16>(at, live, f);
-  else store_vec<BF16>(at, live, f);
-}
 __device__ __forceinline__ void load_params(const AddNormLaunch &p, const void *v, float none, int column, int live, float (&f)[kVec]) {
 #pragma unroll
   for (int c = 0; c < kVec; ++c) f[c] = none;
   if (v == nullptr || live == 0) return;
+  const char *at = static_cast<const char *>(v) + (long long)column * bytes_of(p.param_dtype);
   Raw r = {};
-  load_any(p.param_dtype, static_cast<const char *>(v) + (long long)column * bytes_of(p.param_dtype), live, r);
-  decode_any(p.param_dtype, r, f);
+  if (p.param_dtype == F32::kCode) {
+    load_vec<F32>(at, live, r);
+    decode_vec<F32>(r, f);
+  } else {
+    load_vec<F16>(at, live, r);
+    if (p.param_dtype == F16::kCode) decode_vec<F16>(r, f);
+    else decode_vec<BF16>(r, f);
+  }
 }
+template <typename Tag>
+__device__ __forceinline__ char *element(const void *base, long long i) { return static_cast<char *>(const_cast<void *>(base)) + i * Tag::kBytes; }
 
 // Sums over a team of lanes.  A team that is a whole workgroup of several waves meets in LDS; two sets of slots in turn, so one
 // barrier a sum is enough.
+constexpr int kMostWaves = 8;
 template <int N>
-__device__ __forceinline__ void team_sum(float (&v)[N], int team, float (*slots)[16][2], int &turn) {
+__device__ __forceinline__ void team_sum(float (&v)[N], int team, float (*slots)[kMostWaves][2], int &turn) {
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = cluster_sum(v[i], team < kWave ? team : kWave);
   if (team <= kWave) return;
@@ -128,122 +124,182 @@ struct Geometry {
   unsigned blocks;
 };
 
-// What a lane reads of a row: x and, where there is one, the residual.
-template <typename X, typename R>
-struct RowLoads {
+// X, R: the summands' types (R may be None); the sum has the wider one's, the result as well or, WIDE, fp32.  V: vectors a lane.
+template <typename X_, typename R_, bool WIDE, int V_>
+struct Types {
+  typedef X_ X;
+  typedef R_ R;
   static constexpr bool kSum = !std::is_same_v<R, None>;
-  Raw x, r;
-  __device__ __forceinline__ void request(const AddNormLaunch &p, long long row, int column, int live) {
-    x = {};
-    r = {};
-    if (live == 0) return;
-    load_vec<X>(static_cast<const char *>(p.x.base) + (row * p.x.pitch + column) * X::kBytes, live, x);
-    if constexpr (kSum) load_vec<R>(static_cast<const char *>(p.residual.base) + (row * p.residual.pitch + column) * R::kBytes, live, r);
-  }
-  __device__ __forceinline__ void sum(float (&z)[kVec]) const {
-    decode_vec<X>(x, z);
-    if constexpr (kSum) {
-      float f[kVec];
-      decode_vec<R>(r, f);
+  typedef std::conditional_t<std::is_same_v<R, F32>, F32, X> Sum;
+  typedef std::conditional_t<WIDE, F32, Sum> Out;
+  static constexpr int V = V_;
+};
+
+// What a lane reads of a row: x and, where there is one, the residual.
+template <typename T>
+struct RowLoads {
+  Raw x[T::V], r[T::V];
+  __device__ __forceinline__ void request(const AddNormLaunch &p, long long row, const int (&column)[T::V], const int (&live)[T::V]) {
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) z[c] += f[c];
+    for (int u = 0; u < T::V; ++u) {
+      x[u] = {};
+      r[u] = {};
+      if (live[u] == 0) continue;
+      load_vec<typename T::X>(element<typename T::X>(p.x.base, row * p.x.pitch + column[u]), live[u], x[u]);
+      if constexpr (T::kSum) load_vec<typename T::R>(element<typename T::R>(p.residual.base, row * p.residual.pitch + column[u]), live[u], r[u]);
+    }
+  }
+  __device__ __forceinline__ void sum(float (&z)[T::V][kVec]) const {
+#pragma unroll
+    for (int u = 0; u < T::V; ++u) {
+      decode_vec<typename T::X>(x[u], z[u]);
+      if constexpr (T::kSum) {
+        float f[kVec];
+        decode_vec<typename T::R>(r[u], f);
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) z[u][c] += f[c];
+      }
     }
   }
 };
 
-template <typename X, typename R, int THREADS>
-__global__ void __launch_bounds__(THREADS) add_norm_forward_kernel(const AddNormLaunch p, const Geometry g) {
-  __shared__ float s_slots[2][16][2];
+constexpr int kMostThreads = kMostWaves * kWave;
+template <typename T>
+__global__ void __launch_bounds__(kMostThreads) add_norm_forward_kernel(const AddNormLaunch p, const Geometry g) {
+  constexpr int V = T::V;
+  __shared__ float s_slots[2][kMostWaves][2];
   int turn = 0;
-  const int teams = (int)blockDim.x / g.team, mine = threadIdx.x / g.team, column = (threadIdx.x & (g.team - 1)) * kVec;
-  const int width_live = min(kVec, max(0, p.width - column));
+  const int teams = (int)blockDim.x / g.team, mine = threadIdx.x / g.team;
+  int column[V], width_live[V], none[V];
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    column[u] = ((threadIdx.x & (g.team - 1)) + u * g.team) * kVec;
+    width_live[u] = min(kVec, max(0, p.width - column[u]));
+    none[u] = 0;
+  }
   const float inv = 1.f / (float)p.width;
   const long long begin = blockIdx.x * g.slab, end = min(begin + g.slab, p.rows);
-  RowLoads<X, R> next;
-  next.request(p, begin + mine, column, begin + mine < end ? width_live : 0);
-  float w[kVec], b[kVec];
-  load_params(p, p.weight, 1.f, column, width_live, w);
-  load_params(p, p.bias, 0.f, column, width_live, b);
+  RowLoads<T> next;
+  next.request(p, begin + mine, column, begin + mine < end ? width_live : none);
+  float w[V][kVec], b[V][kVec];
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    load_params(p, p.weight, 1.f, column[u], width_live[u], w[u]);
+    load_params(p, p.bias, 0.f, column[u], width_live[u], b[u]);
+  }
   for (long long row0 = begin; row0 < end; row0 += teams) {
     const long long row = row0 + mine;
-    const int live = row < end ? width_live : 0;
-    float z[kVec];
+    float z[V][kVec];
     next.sum(z);
-    next.request(p, row + teams, column, row + teams < end ? width_live : 0);
+    next.request(p, row + teams, column, row + teams < end ? width_live : none);
     float sum[1] = {0.f};
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) sum[0] += z[c];      // zeros beyond the width
+    for (int u = 0; u < V; ++u)
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) sum[0] += z[u][c];      // zeros beyond the width
     team_sum(sum, g.team, s_slots, turn);
     const float mean = sum[0] * inv;
     float squares[1] = {0.f};
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) squares[0] = c < live ? fmaf(z[c] - mean, z[c] - mean, squares[0]) : squares[0];
+    for (int u = 0; u < V; ++u)
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) squares[0] = c < width_live[u] ? fmaf(z[u][c] - mean, z[u][c] - mean, squares[0]) : squares[0];
     team_sum(squares, g.team, s_slots, turn);
     const float rstd = 1.f / sqrtf(fmaf(squares[0], inv, p.eps));
-    if (live == 0) continue;
-    if (p.sum != nullptr) store_any(p.sum_dtype, p.sum, row * p.width + column, live, z);
-    if (p.stats != nullptr && column == 0) reinterpret_cast<f32x2 *>(p.stats)[row] = f32x2{mean, rstd};
+    if (row >= end) continue;
+    if (p.stats != nullptr && column[0] == 0) reinterpret_cast<f32x2 *>(p.stats)[row] = f32x2{mean, rstd};
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) z[c] = fmaf((z[c] - mean) * rstd, w[c], b[c]);
-    store_any(p.out_dtype, p.out, row * p.width + column, live, z);
+    for (int u = 0; u < V; ++u) {
+      if (width_live[u] == 0) continue;
+      const long long at = row * p.width + column[u];
+      if (p.sum != nullptr) store_vec<typename T::Sum>(element<typename T::Sum>(p.sum, at), width_live[u], z[u]);
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) z[u][c] = fmaf((z[u][c] - mean) * rstd, w[u][c], b[u][c]);
+      store_vec<typename T::Out>(element<typename T::Out>(p.out, at), width_live[u], z[u]);
+    }
   }
 }
 
-template <typename X, typename R, int THREADS>
-__global__ void __launch_bounds__(THREADS) add_norm_backward_kernel(const AddNormLaunch p, const Geometry g) {
+template <typename T>
+__global__ void __launch_bounds__(kMostThreads) add_norm_backward_kernel(const AddNormLaunch p, const Geometry g) {
+  constexpr int V = T::V;
+  typedef typename T::Out Out;
+  typedef typename T::Sum Sum;
   extern __shared__ float s_columns[];      // [teams][vectors * 8]
-  __shared__ float s_slots[2][16][2];
+  __shared__ float s_slots[2][kMostWaves][2];
   int turn = 0;
-  const int teams = (int)blockDim.x / g.team, mine = threadIdx.x / g.team, column = (threadIdx.x & (g.team - 1)) * kVec;
-  const int width_live = min(kVec, max(0, p.width - column));
+  const int teams = (int)blockDim.x / g.team, mine = threadIdx.x / g.team;
+  int column[V], width_live[V], none[V];
+#pragma unroll
+  for (int u = 0; u < V; ++u) {
+    column[u] = ((threadIdx.x & (g.team - 1)) + u * g.team) * kVec;
+    width_live[u] = min(kVec, max(0, p.width - column[u]));
+    none[u] = 0;
+  }
   const float inv = 1.f / (float)p.width;
   const long long begin = blockIdx.x * g.slab, end = min(begin + g.slab, p.rows);
-  RowLoads<X, R> next;
-  Raw next_g, next_s;
+  RowLoads<T> next;
+  Raw next_g[V], next_s[V];
   f32x2 next_stats;
   auto request = [&](long long row) {
-    const int live = row < end ? width_live : 0;
-    next.request(p, row, column, live);
-    next_g = {};
-    next_s = {};
+    next.request(p, row, column, row < end ? width_live : none);
     next_stats = f32x2{0.f, 0.f};
     if (row < end) next_stats = reinterpret_cast<const f32x2 *>(p.stats)[row];
-    if (live == 0) return;
-    const long long at = row * p.width + column;
-    load_any(p.out_dtype, static_cast<const char *>(p.grad_out) + at * bytes_of(p.out_dtype), live, next_g);
-    if (p.grad_sum != nullptr) load_any(p.sum_dtype, static_cast<const char *>(p.grad_sum) + at * bytes_of(p.sum_dtype), live, next_s);
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      next_g[u] = {};
+      next_s[u] = {};
+      if (row >= end || width_live[u] == 0) continue;
+      const long long at = row * p.width + column[u];
+      load_vec<Out>(element<Out>(p.grad_out, at), width_live[u], next_g[u]);
+      if (p.grad_sum != nullptr) load_vec<Sum>(element<Sum>(p.grad_sum, at), width_live[u], next_s[u]);
+    }
   };
   request(begin + mine);
-  float w[kVec], dw[kVec], db[kVec];
-  load_params(p, p.weight, 1.f, column, width_live, w);
+  float w[V][kVec], dw[V][kVec], db[V][kVec];
 #pragma unroll
-  for (int c = 0; c < kVec; ++c) dw[c] = db[c] = 0.f;
+  for (int u = 0; u < V; ++u) {
+    load_params(p, p.weight, 1.f, column[u], width_live[u], w[u]);
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) dw[u][c] = db[u][c] = 0.f;
+  }
   for (long long row0 = begin; row0 < end; row0 += teams) {
     const long long row = row0 + mine;
-    const int live = row < end ? width_live : 0;
-    float z[kVec], a[kVec], around[kVec];
+    float z[V][kVec], a[V][kVec], around[V][kVec];
     next.sum(z);
-    decode_any(p.out_dtype, next_g, a);
-    decode_any(p.sum_dtype, next_s, around);
-    const float mean = next_stats.x, rstd = next_stats.y;
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      decode_vec<Out>(next_g[u], a[u]);
+      decode_vec<Sum>(next_s[u], around[u]);
+    }
+    const float rstd = next_stats.y, shift = -next_stats.x * rstd;
     request(row + teams);
     float sums[2] = {0.f, 0.f};
+    // beyond the width and the rows the gradients are zeros, and so is all that is added up
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) {
-      z[c] = c < live ? (z[c] - mean) * rstd : 0.f;
-      dw[c] = fmaf(a[c], z[c], dw[c]);
-      db[c] += a[c];
-      a[c] *= w[c];
-      sums[0] += a[c];
-      sums[1] = fmaf(a[c], z[c], sums[1]);
-    }
+    for (int u = 0; u < V; ++u)
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) {
+        z[u][c] = fmaf(z[u][c], rstd, shift);
+        dw[u][c] = fmaf(a[u][c], z[u][c], dw[u][c]);
+        db[u][c] += a[u][c];
+        a[u][c] *= w[u][c];
+        sums[0] += a[u][c];
+        sums[1] = fmaf(a[u][c], z[u][c], sums[1]);
+      }
     team_sum(sums, g.team, s_slots, turn);
-    if (live == 0) continue;
+    if (row >= end) continue;
     const float m1 = sums[0] * inv, m2 = sums[1] * inv;
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) a[c] = fmaf(rstd, a[c] - m1 - z[c] * m2, around[c]);
-    if (p.grad_x != nullptr) store_any(p.grad_x_dtype, p.grad_x, row * p.width + column, live, a);
-    if (p.grad_residual != nullptr) store_any(p.grad_residual_dtype, p.grad_residual, row * p.width + column, live, a);
+    for (int u = 0; u < V; ++u) {
+      if (width_live[u] == 0) continue;
+      const long long at = row * p.width + column[u];
+#pragma unroll
+      for (int c = 0; c < kVec; ++c) a[u][c] = fmaf(rstd, a[u][c] - m1 - z[u][c] * m2, around[u][c]);
+      if (p.grad_x != nullptr) store_vec<typename T::X>(element<typename T::X>(p.grad_x, at), width_live[u], a[u]);
+      if constexpr (T::kSum)
+        if (p.grad_residual != nullptr) store_vec<typename T::R>(element<typename T::R>(p.grad_residual, at), width_live[u], a[u]);
+    }
   }
   if (p.grad_weight == nullptr && p.grad_bias == nullptr) return;
   const int padded = (p.width + kVec - 1) / kVec * kVec;
@@ -251,9 +307,11 @@ __global__ void __launch_bounds__(THREADS) add_norm_backward_kernel(const AddNor
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     __syncthreads();
-    if (width_live > 0)
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) s_columns[(size_t)mine * padded + column + c] = q == 0 ? dw[c] : db[c];
+    for (int u = 0; u < V; ++u)
+      if (width_live[u] > 0)
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) s_columns[(size_t)mine * padded + column[u] + c] = q == 0 ? dw[u][c] : db[u][c];
     __syncthreads();
     for (int c = threadIdx.x; c < padded; c += blockDim.x) {
       float sum = 0.f;
@@ -289,17 +347,23 @@ __global__ void __launch_bounds__(kGradColumns * kGradLanes) add_norm_param_grad
   float total[kVec] = {};
 #pragma unroll
   for (int l = 0; l < kGradLanes; ++l) total[0] += s_part[l][c];
-  store_any(p.param_dtype, to, column, 1, total);
+  char *at = static_cast<char *>(to) + (long long)column * bytes_of(p.param_dtype);
+  if (p.param_dtype == F32::kCode) store_vec<F32>(at, 1, total);
+  else if (p.param_dtype == F16::kCode) store_vec<F16>(at, 1, total);
+  else store_vec<BF16>(at, 1, total);
 }
 
+// A lane has two vectors of rows of more than 64, so that a wave holds a row of up to 1024 channels and meets no barrier.
+int vectors_of(const AddNormLaunch &p) { return (p.width + kVec - 1) / kVec; }
+bool two_a_lane(const AddNormLaunch &p) { return vectors_of(p) > kWave; }
 // Parameters in registers pay over several rows; workgroups enough to fill the chip come first.
 Geometry geometry(const AddNormLaunch &p, long long most_blocks) {
   Geometry g;
-  const int vectors = (p.width + kVec - 1) / kVec;
+  const int vectors = (vectors_of(p) + two_a_lane(p)) / (two_a_lane(p) ? 2 : 1);
   g.team = 1;
   while (g.team < vectors) g.team *= 2;
   g.threads = std::max(g.team, 64);
-  if (g.team < 256 && g.team <= kWave && p.rows * g.team >= 256ll * 1024) g.threads = 256;
+  if (g.team <= kWave && p.rows * g.team >= 256ll * 1024) g.threads = 256;
   const long long teams = g.threads / g.team, passes = (p.rows + teams - 1) / teams;
   const long long blocks = std::min(passes, most_blocks);
   g.slab = (passes + blocks - 1) / blocks * teams;
@@ -309,37 +373,42 @@ Geometry geometry(const AddNormLaunch &p, long long most_blocks) {
 Geometry forward_geometry(const AddNormLaunch &p) { return geometry(p, 4096); }
 Geometry backward_geometry(const AddNormLaunch &p) {
   // partial sums stay below 32 MB
-  const long long columns = (p.width + kVec - 1) / kVec * kVec;
+  const long long columns = (long long)vectors_of(p) * kVec;
   return geometry(p, std::max<long long>(1, std::min<long long>(1024, (32ll << 20) / (8 * columns))));
 }
 
-template <typename X, typename R>
-hipError_t forward_t(const AddNormLaunch &p, hipStream_t stream) {
-  const Geometry g = forward_geometry(p);
-  if (g.threads <= 256) hipLaunchKernelGGL((add_norm_forward_kernel<X, R, 256>), dim3(g.blocks), dim3(g.threads), 0, stream, p, g);
-  else hipLaunchKernelGGL((add_norm_forward_kernel<X, R, 1024>), dim3(g.blocks), dim3(g.threads), 0, stream, p, g);
-  return hipGetLastError();
-}
-template <typename X, typename R>
-hipError_t backward_t(const AddNormLaunch &p, hipStream_t stream) {
+template <typename T>
+hipError_t run(const AddNormLaunch &p, hipStream_t stream, bool backward) {
+  if (!backward) {
+    const Geometry g = forward_geometry(p);
+    hipLaunchKernelGGL((add_norm_forward_kernel<T>), dim3(g.blocks), dim3(g.threads), 0, stream, p, g);
+    return hipGetLastError();
+  }
   const Geometry g = backward_geometry(p);
-  const int padded = (p.width + kVec - 1) / kVec * kVec;
+  const int padded = vectors_of(p) * kVec;
   const size_t lds = (size_t)(g.threads / g.team) * padded * sizeof(float);
-  if (g.threads <= 256) hipLaunchKernelGGL((add_norm_backward_kernel<X, R, 256>), dim3(g.blocks), dim3(g.threads), lds, stream, p, g);
-  else hipLaunchKernelGGL((add_norm_backward_kernel<X, R, 1024>), dim3(g.blocks), dim3(g.threads), lds, stream, p, g);
+  hipLaunchKernelGGL((add_norm_backward_kernel<T>), dim3(g.blocks), dim3(g.threads), lds, stream, p, g);
   if (hipError_t e = hipGetLastError()) return e;
   if (p.grad_weight == nullptr && p.grad_bias == nullptr) return hipSuccess;
   hipLaunchKernelGGL(add_norm_param_grad_kernel, dim3((2 * padded + kGradColumns - 1) / kGradColumns), dim3(kGradColumns * kGradLanes), 0, stream, p, g.blocks);
   return hipGetLastError();
 }
-
+template <typename X, typename R, bool WIDE>
+hipError_t with_types(const AddNormLaunch &p, hipStream_t stream, bool backward) {
+  return two_a_lane(p) ? run<Types<X, R, WIDE, 2>>(p, stream, backward) : run<Types<X, R, WIDE, 1>>(p, stream, backward);
+}
 template <typename X>
 hipError_t with_residual(const AddNormLaunch &p, hipStream_t stream, bool backward) {
-  if (p.residual.base == nullptr) return backward ? backward_t<X, None>(p, stream) : forward_t<X, None>(p, stream);
-  if (p.residual.dtype == X::kCode) return backward ? backward_t<X, X>(p, stream) : forward_t<X, X>(p, stream);
-  if constexpr (X::kCode != F32::kCode)
-    if (p.residual.dtype == F32::kCode) return backward ? backward_t<X, F32>(p, stream) : forward_t<X, F32>(p, stream);
-  return hipErrorInvalidValue;
+  const bool none = p.residual.base == nullptr;
+  if constexpr (X::kCode == F32::kCode) {
+    if (none) return with_types<X, None, false>(p, stream, backward);
+    return p.residual.dtype == X::kCode ? with_types<X, X, false>(p, stream, backward) : hipErrorInvalidValue;
+  } else {
+    if (none) return p.wide ? with_types<X, None, true>(p, stream, backward) : with_types<X, None, false>(p, stream, backward);
+    if (p.residual.dtype == F32::kCode) return with_types<X, F32, false>(p, stream, backward);
+    if (p.residual.dtype != X::kCode) return hipErrorInvalidValue;
+    return p.wide ? with_types<X, X, true>(p, stream, backward) : with_types<X, X, false>(p, stream, backward);
+  }
 }
 hipError_t launch(const AddNormLaunch &p, hipStream_t stream, bool backward) {
   if (p.rows <= 0 || p.width <= 0 || p.width > kMaxNormWidth) return hipErrorInvalidValue;
@@ -355,7 +424,7 @@ hipError_t launch(const AddNormLaunch &p, hipStream_t stream, bool backward) {
 
 size_t add_norm_backward_workspace_bytes(const AddNormLaunch &p) {
   if (p.grad_weight == nullptr && p.grad_bias == nullptr) return 0;
-  return (size_t)backward_geometry(p).blocks * 2 * ((p.width + kVec - 1) / kVec * kVec) * sizeof(float);
+  return (size_t)backward_geometry(p).blocks * 2 * vectors_of(p) * kVec * sizeof(float);
 }
 hipError_t launch_add_norm_forward(const AddNormLaunch &p, hipStream_t stream) { return launch(p, stream, false); }
 hipError_t launch_add_norm_backward(const AddNormLaunch &p, hipStream_t stream) { return launch(p, stream, true); }

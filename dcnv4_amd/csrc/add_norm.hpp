@@ -21,13 +21,12 @@ struct AddNormLaunch {
   long long rows;
   int width;
   float eps;
-  void *out, *sum;                // dense; the sum may be null
-  int out_dtype, sum_dtype;
+  bool wide;                      // a result in fp32 whatever the summands
+  void *out, *sum;                // dense; the sum, of the summands' wider type, may be null
   float *stats;                   // (rows, 2): mean and 1 / deviation; the forward writes them where they are wanted
   // backward: x, residual, stats and
   const void *grad_out, *grad_sum;                  // dense, of the outputs' types; grad_sum may be null
-  void *grad_x, *grad_residual;                     // dense; grad_residual may be null
-  int grad_x_dtype, grad_residual_dtype;
+  void *grad_x, *grad_residual;                     // dense, of the summands' types; each may be null
   void *grad_weight, *grad_bias;                    // each may be null
   void *workspace;
 };

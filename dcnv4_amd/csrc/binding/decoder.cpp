@@ -296,11 +296,13 @@ Tensor rows_of(const Tensor &t) {
 struct NormCall {
   Tensor x, residual, weight, bias;
   AddNormLaunch l = {};
+  bool turned = false;      // x and residual have changed places
 
   explicit NormCall(const NormInputs &a) : x(rows_of(a.x)) {
     if (a.residual.defined()) residual = rows_of(a.residual);
     // the kernel wants the fp32 one of two types second
-    if (residual.defined() && x.scalar_type() != residual.scalar_type() && x.scalar_type() == at::kFloat) std::swap(x, residual);
+    turned = residual.defined() && x.scalar_type() != residual.scalar_type() && x.scalar_type() == at::kFloat;
+    if (turned) std::swap(x, residual);
     if (a.weight.defined()) weight = a.weight.contiguous();
     if (a.bias.defined()) bias = a.bias.contiguous();
     l.x = view(x);
@@ -310,8 +312,7 @@ struct NormCall {
     l.rows = x.size(0);
     l.width = (int)x.size(1);
     l.eps = a.eps;
-    l.out_dtype = code(a.out_dtype());
-    l.sum_dtype = code(a.sum_dtype());
+    l.wide = a.wide;
   }
   static int code(at::ScalarType t) { return t == at::kFloat ? DCNV4_DTYPE_F32 : t == at::kHalf ? DCNV4_DTYPE_F16 : DCNV4_DTYPE_BF16; }
 
@@ -359,15 +360,11 @@ std::array<Tensor, 4> norm_backward(const NormInputs &a, const Tensor &stats, co
     NormCall c(a);
     const Tensor g = grad_out.contiguous(), s = grad_sum.defined() ? grad_sum.contiguous() : grad_sum, kept = stats.contiguous();
     c.l.stats = kept.data_ptr<float>();
-    c.l.out_dtype = NormCall::code(g.scalar_type());
-    c.l.sum_dtype = NormCall::code(sum_dtype);
     c.l.grad_out = g.data_ptr();
     c.l.grad_sum = ptr(s);
     c.l.grad_x = ptr(grads[0]);
-    c.l.grad_x_dtype = NormCall::code(x_dtype);
-    const bool apart = grads[1].defined() && !grads[1].is_same(grads[0]);
-    c.l.grad_residual = apart ? ptr(grads[1]) : nullptr;
-    c.l.grad_residual_dtype = NormCall::code(residual_dtype);
+    c.l.grad_residual = grads[1].is_same(grads[0]) ? nullptr : ptr(grads[1]);
+    if (c.turned) std::swap(c.l.grad_x, c.l.grad_residual);
     c.l.grad_weight = ptr(grads[2]); c.l.grad_bias = ptr(grads[3]);
     const Tensor ws = workspace(add_norm_backward_workspace_bytes(c.l), a.x);
     c.l.workspace = ptr(ws);
