@@ -4,11 +4,15 @@
 //   dz = rstd (a - mean(a) - xhat mean(a xhat)) + grad_sum,   dweight = sum over rows of grad_out xhat,   dbias = sum of grad_out
 //
 // HBM-bound: each tensor is read or written once.  A team of lanes (a power of two, up to a whole workgroup of 512) owns a row, a
-// lane eight or twice eight elements of it, which stay in registers as fp32 from the sum to the result: the sum is not rounded
+// lane eight or sixteen elements of it, which stay in registers as fp32 from the sum to the result: the sum is not rounded
 // before it is normalised.  The mean and the deviations about it are two reductions over the team; both are kept for the
-// backward, 8 bytes a row, which then reduces once.  A workgroup walks a slab of rows with the parameters in registers and the next
-// row's loads under way.  A row may start at any element and have any width: the loads are unaligned ones, the last
-// elements of a width that is no multiple of eight are read and written one by one.
+// backward, 8 bytes a row, which then reduces once.  A workgroup walks a slab of rows with the parameters in registers and the loads of the
+// next under way.
+//
+// Rows that all start on 16 bytes go in vectors of eight elements.  Others (an odd width, an odd offset) go element by element, neighbours
+// in neighbouring lanes: a 16-byte access that crosses its alignment costs twice (100000 x 1023, 16 bits, forward 283 us and backward 589
+// in unaligned vectors, 200 and 251 so; 1024 channels 148 and 228).  The backward reads four tensors for the one it writes, which
+// memory gives at some 4.5 TB/s, a copy 6.2; loads two rows ahead were slower (401408 x 112: 112 us for 98).
 //
 // The parameters' gradients are summed in registers down a workgroup's slab, over its teams through LDS, and over the workgroups by a
 // second kernel, always in the same order.
@@ -23,76 +27,36 @@ namespace dcn {
 namespace {
 
 struct None {};
-constexpr int kVec = 8;
 
-struct __attribute__((packed, aligned(2))) Unaligned { u32x4 v; };
-struct Raw { u32x4 w[2]; };      // eight elements; of a 16-bit type in w[0]
-
-template <typename Tag>
-__device__ __forceinline__ void load_vec(const char *at, int live, Raw &r) {
-  if (live == kVec) {
+// One access: G consecutive elements, eight or one.
+template <typename Tag, int G> struct Access {
+  static constexpr int kWords = G * Tag::kBytes > 16 ? 2 : 1;
+  typedef Pack<Tag, G / kWords> pack_t;
+  struct raw_t { typename pack_t::raw_t w[kWords]; };
+  static __device__ __forceinline__ raw_t load(const char *at) { return *reinterpret_cast<const raw_t *>(at); }
+  static __device__ __forceinline__ void decode(const raw_t &r, float (&f)[G]) {
 #pragma unroll
-    for (int i = 0; i < Tag::kBytes / 2; ++i) r.w[i] = reinterpret_cast<const Unaligned *>(at)[i].v;
-    return;
-  }
-  if constexpr (Tag::kBytes == 4) {
+    for (int i = 0; i < kWords; ++i) {
+      float part[G / kWords];
+      pack_t::decode(r.w[i], part);
 #pragma unroll
-    for (int c = 0; c < kVec; ++c)
-      if (c < live) r.w[c / 4][c % 4] = reinterpret_cast<const uint32_t *>(at)[c];
-  } else {
-#pragma unroll
-    for (int c = 0; c < kVec; ++c)
-      if (c < live) r.w[0][c / 2] |= (uint32_t)reinterpret_cast<const uint16_t *>(at)[c] << (c % 2 * 16);
-  }
-}
-template <typename Tag>
-__device__ __forceinline__ void decode_vec(const Raw &r, float (&f)[kVec]) {
-  if constexpr (Tag::kBytes == 4) {
-    float a[4], b[4];
-    Pack<Tag, 4>::decode(r.w[0], a);
-    Pack<Tag, 4>::decode(r.w[1], b);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) { f[c] = a[c]; f[4 + c] = b[c]; }
-  } else {
-    Pack<Tag, 8>::decode(r.w[0], f);
-  }
-}
-template <typename Tag>
-__device__ __forceinline__ void store_vec(char *at, int live, const float (&f)[kVec]) {
-  if (live == kVec) {
-    if constexpr (Tag::kBytes == 4) {
-      const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
-      reinterpret_cast<Unaligned *>(at)[0].v = Pack<Tag, 4>::encode(a);
-      reinterpret_cast<Unaligned *>(at)[1].v = Pack<Tag, 4>::encode(b);
-    } else {
-      reinterpret_cast<Unaligned *>(at)->v = Pack<Tag, 8>::encode(f);
+      for (int c = 0; c < G / kWords; ++c) f[i * (G / kWords) + c] = part[c];
     }
-    return;
   }
+  static __device__ __forceinline__ void store(char *at, const float (&f)[G]) {
+    raw_t r;
 #pragma unroll
-  for (int c = 0; c < kVec; ++c)
-    if (c < live) {
-      const float one[1] = {f[c]};
-      reinterpret_cast<typename RawWord<Tag::kBytes>::type *>(at)[c] = Pack<Tag, 1>::encode(one);
+    for (int i = 0; i < kWords; ++i) {
+      float part[G / kWords];
+#pragma unroll
+      for (int c = 0; c < G / kWords; ++c) part[c] = f[i * (G / kWords) + c];
+      r.w[i] = pack_t::encode(part);
     }
-}
+    *reinterpret_cast<raw_t *>(at) = r;
+  }
+};
 // Parameters go by their type's code, one for all lanes.
 __device__ __forceinline__ int bytes_of(int dtype) { return dtype == F32::kCode ? 4 : 2; }
-__device__ __forceinline__ void load_params(const AddNormLaunch &p, const void *v, float none, int column, int live, float (&f)[kVec]) {
-#pragma unroll
-  for (int c = 0; c < kVec; ++c) f[c] = none;
-  if (v == nullptr || live == 0) return;
-  const char *at = static_cast<const char *>(v) + (long long)column * bytes_of(p.param_dtype);
-  Raw r = {};
-  if (p.param_dtype == F32::kCode) {
-    load_vec<F32>(at, live, r);
-    decode_vec<F32>(r, f);
-  } else {
-    load_vec<F16>(at, live, r);
-    if (p.param_dtype == F16::kCode) decode_vec<F16>(r, f);
-    else decode_vec<BF16>(r, f);
-  }
-}
 template <typename Tag>
 __device__ __forceinline__ char *element(const void *base, long long i) { return static_cast<char *>(const_cast<void *>(base)) + i * Tag::kBytes; }
 
@@ -124,214 +88,241 @@ struct Geometry {
   unsigned blocks;
 };
 
-// X, R: the summands' types (R may be None); the sum has the wider one's, the result as well or, WIDE, fp32.  V: vectors a lane.
-template <typename X_, typename R_, bool WIDE, int V_>
+// X, R: the summands' types (R may be None); the sum has the wider one's, the result as well or, WIDE, fp32.  A lane makes N accesses
+// of G elements a row.
+template <typename X_, typename R_, bool WIDE, int G_, int N_>
 struct Types {
   typedef X_ X;
   typedef R_ R;
   static constexpr bool kSum = !std::is_same_v<R, None>;
   typedef std::conditional_t<std::is_same_v<R, F32>, F32, X> Sum;
   typedef std::conditional_t<WIDE, F32, Sum> Out;
-  static constexpr int V = V_;
+  static constexpr int G = G_, N = N_;
+};
+
+// The columns of a lane.
+template <typename T>
+struct Columns {
+  int at[T::N];
+  bool live[T::N];
+  __device__ __forceinline__ Columns(int team, int width) {
+#pragma unroll
+    for (int n = 0; n < T::N; ++n) {
+      at[n] = ((threadIdx.x & (team - 1)) + n * team) * T::G;
+      live[n] = at[n] < width;
+    }
+  }
 };
 
 // What a lane reads of a row: x and, where there is one, the residual.
 template <typename T>
 struct RowLoads {
-  Raw x[T::V], r[T::V];
-  __device__ __forceinline__ void request(const AddNormLaunch &p, long long row, const int (&column)[T::V], const int (&live)[T::V]) {
+  typedef Access<typename T::X, T::G> ax;
+  typedef Access<std::conditional_t<T::kSum, typename T::R, typename T::X>, T::G> ar;
+  typename ax::raw_t x[T::N];
+  typename ar::raw_t r[T::N];
+  __device__ __forceinline__ void request(const AddNormLaunch &p, long long row, const Columns<T> &c, bool there) {
 #pragma unroll
-    for (int u = 0; u < T::V; ++u) {
-      x[u] = {};
-      r[u] = {};
-      if (live[u] == 0) continue;
-      load_vec<typename T::X>(element<typename T::X>(p.x.base, row * p.x.pitch + column[u]), live[u], x[u]);
-      if constexpr (T::kSum) load_vec<typename T::R>(element<typename T::R>(p.residual.base, row * p.residual.pitch + column[u]), live[u], r[u]);
+    for (int n = 0; n < T::N; ++n) {
+      x[n] = {};
+      r[n] = {};
+      if (!there || !c.live[n]) continue;
+      x[n] = ax::load(element<typename T::X>(p.x.base, row * p.x.pitch + c.at[n]));
+      if constexpr (T::kSum) r[n] = ar::load(element<typename T::R>(p.residual.base, row * p.residual.pitch + c.at[n]));
     }
   }
-  __device__ __forceinline__ void sum(float (&z)[T::V][kVec]) const {
+  __device__ __forceinline__ void sum(float (&z)[T::N][T::G]) const {
 #pragma unroll
-    for (int u = 0; u < T::V; ++u) {
-      decode_vec<typename T::X>(x[u], z[u]);
+    for (int n = 0; n < T::N; ++n) {
+      ax::decode(x[n], z[n]);
       if constexpr (T::kSum) {
-        float f[kVec];
-        decode_vec<typename T::R>(r[u], f);
+        float f[T::G];
+        ar::decode(r[n], f);
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) z[u][c] += f[c];
+        for (int c = 0; c < T::G; ++c) z[n][c] += f[c];
       }
     }
   }
 };
 
+template <typename T, typename Tag>
+__device__ __forceinline__ void load_params(const void *v, const Columns<T> &column, float (&f)[T::N][T::G]) {
+  typename Access<Tag, T::G>::raw_t r[T::N];
+#pragma unroll
+  for (int n = 0; n < T::N; ++n)
+    if (column.live[n]) r[n] = Access<Tag, T::G>::load(element<Tag>(v, column.at[n]));
+#pragma unroll
+  for (int n = 0; n < T::N; ++n)
+    if (column.live[n]) Access<Tag, T::G>::decode(r[n], f[n]);
+}
+template <typename T>
+__device__ __forceinline__ void load_params(const AddNormLaunch &p, const void *v, float none, const Columns<T> &column, float (&f)[T::N][T::G]) {
+#pragma unroll
+  for (int n = 0; n < T::N; ++n)
+#pragma unroll
+    for (int c = 0; c < T::G; ++c) f[n][c] = none;
+  if (v == nullptr) return;
+  if (p.param_dtype == F32::kCode) load_params<T, F32>(v, column, f);
+  else if (p.param_dtype == F16::kCode) load_params<T, F16>(v, column, f);
+  else load_params<T, BF16>(v, column, f);
+}
+
 constexpr int kMostThreads = kMostWaves * kWave;
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads) add_norm_forward_kernel(const AddNormLaunch p, const Geometry g) {
-  constexpr int V = T::V;
+  constexpr int N = T::N, G = T::G;
   __shared__ float s_slots[2][kMostWaves][2];
   int turn = 0;
   const int teams = (int)blockDim.x / g.team, mine = threadIdx.x / g.team;
-  int column[V], width_live[V], none[V];
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
-    column[u] = ((threadIdx.x & (g.team - 1)) + u * g.team) * kVec;
-    width_live[u] = min(kVec, max(0, p.width - column[u]));
-    none[u] = 0;
-  }
+  const Columns<T> column(g.team, p.width);
   const float inv = 1.f / (float)p.width;
   const long long begin = blockIdx.x * g.slab, end = min(begin + g.slab, p.rows);
   RowLoads<T> next;
-  next.request(p, begin + mine, column, begin + mine < end ? width_live : none);
-  float w[V][kVec], b[V][kVec];
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
-    load_params(p, p.weight, 1.f, column[u], width_live[u], w[u]);
-    load_params(p, p.bias, 0.f, column[u], width_live[u], b[u]);
-  }
+  next.request(p, begin + mine, column, begin + mine < end);
+  float w[N][G], b[N][G];
+  load_params<T>(p, p.weight, 1.f, column, w);
+  load_params<T>(p, p.bias, 0.f, column, b);
   for (long long row0 = begin; row0 < end; row0 += teams) {
     const long long row = row0 + mine;
-    float z[V][kVec];
+    float z[N][G];
     next.sum(z);
-    next.request(p, row + teams, column, row + teams < end ? width_live : none);
+    next.request(p, row + teams, column, row + teams < end);
     float sum[1] = {0.f};
 #pragma unroll
-    for (int u = 0; u < V; ++u)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) sum[0] += z[u][c];      // zeros beyond the width
+      for (int c = 0; c < G; ++c) sum[0] += z[n][c];      // zeros beyond the width
     team_sum(sum, g.team, s_slots, turn);
     const float mean = sum[0] * inv;
     float squares[1] = {0.f};
 #pragma unroll
-    for (int u = 0; u < V; ++u)
+    for (int n = 0; n < N; ++n) {
+      float own = squares[0];
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) squares[0] = c < width_live[u] ? fmaf(z[u][c] - mean, z[u][c] - mean, squares[0]) : squares[0];
+      for (int c = 0; c < G; ++c) own = fmaf(z[n][c] - mean, z[n][c] - mean, own);
+      squares[0] = column.live[n] ? own : squares[0];
+    }
     team_sum(squares, g.team, s_slots, turn);
     const float rstd = 1.f / sqrtf(fmaf(squares[0], inv, p.eps));
     if (row >= end) continue;
-    if (p.stats != nullptr && column[0] == 0) reinterpret_cast<f32x2 *>(p.stats)[row] = f32x2{mean, rstd};
+    if (p.stats != nullptr && column.at[0] == 0) reinterpret_cast<f32x2 *>(p.stats)[row] = f32x2{mean, rstd};
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      if (width_live[u] == 0) continue;
-      const long long at = row * p.width + column[u];
-      if (p.sum != nullptr) store_vec<typename T::Sum>(element<typename T::Sum>(p.sum, at), width_live[u], z[u]);
+    for (int n = 0; n < N; ++n) {
+      if (!column.live[n]) continue;
+      const long long at = row * p.width + column.at[n];
+      if (p.sum != nullptr) Access<typename T::Sum, G>::store(element<typename T::Sum>(p.sum, at), z[n]);
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) z[u][c] = fmaf((z[u][c] - mean) * rstd, w[u][c], b[u][c]);
-      store_vec<typename T::Out>(element<typename T::Out>(p.out, at), width_live[u], z[u]);
+      for (int c = 0; c < G; ++c) z[n][c] = fmaf((z[n][c] - mean) * rstd, w[n][c], b[n][c]);
+      Access<typename T::Out, G>::store(element<typename T::Out>(p.out, at), z[n]);
     }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads) add_norm_backward_kernel(const AddNormLaunch p, const Geometry g) {
-  constexpr int V = T::V;
+  constexpr int N = T::N, G = T::G;
   typedef typename T::Out Out;
   typedef typename T::Sum Sum;
-  extern __shared__ float s_columns[];      // [teams][vectors * 8]
+  extern __shared__ float s_columns[];      // [teams][width]
   __shared__ float s_slots[2][kMostWaves][2];
   int turn = 0;
   const int teams = (int)blockDim.x / g.team, mine = threadIdx.x / g.team;
-  int column[V], width_live[V], none[V];
-#pragma unroll
-  for (int u = 0; u < V; ++u) {
-    column[u] = ((threadIdx.x & (g.team - 1)) + u * g.team) * kVec;
-    width_live[u] = min(kVec, max(0, p.width - column[u]));
-    none[u] = 0;
-  }
+  const Columns<T> column(g.team, p.width);
   const float inv = 1.f / (float)p.width;
   const long long begin = blockIdx.x * g.slab, end = min(begin + g.slab, p.rows);
   RowLoads<T> next;
-  Raw next_g[V], next_s[V];
+  typename Access<Out, G>::raw_t next_g[N];
+  typename Access<Sum, G>::raw_t next_s[N];
   f32x2 next_stats;
   auto request = [&](long long row) {
-    next.request(p, row, column, row < end ? width_live : none);
+    const bool there = row < end;
+    next.request(p, row, column, there);
     next_stats = f32x2{0.f, 0.f};
-    if (row < end) next_stats = reinterpret_cast<const f32x2 *>(p.stats)[row];
+    if (there) next_stats = reinterpret_cast<const f32x2 *>(p.stats)[row];
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      next_g[u] = {};
-      next_s[u] = {};
-      if (row >= end || width_live[u] == 0) continue;
-      const long long at = row * p.width + column[u];
-      load_vec<Out>(element<Out>(p.grad_out, at), width_live[u], next_g[u]);
-      if (p.grad_sum != nullptr) load_vec<Sum>(element<Sum>(p.grad_sum, at), width_live[u], next_s[u]);
+    for (int n = 0; n < N; ++n) {
+      next_g[n] = {};
+      next_s[n] = {};
+      if (!there || !column.live[n]) continue;
+      const long long at = row * p.width + column.at[n];
+      next_g[n] = Access<Out, G>::load(element<Out>(p.grad_out, at));
+      if (p.grad_sum != nullptr) next_s[n] = Access<Sum, G>::load(element<Sum>(p.grad_sum, at));
     }
   };
   request(begin + mine);
-  float w[V][kVec], dw[V][kVec], db[V][kVec];
+  float w[N][G], dw[N][G], db[N][G];
+  load_params<T>(p, p.weight, 1.f, column, w);
 #pragma unroll
-  for (int u = 0; u < V; ++u) {
-    load_params(p, p.weight, 1.f, column[u], width_live[u], w[u]);
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int c = 0; c < kVec; ++c) dw[u][c] = db[u][c] = 0.f;
-  }
+    for (int c = 0; c < G; ++c) dw[n][c] = db[n][c] = 0.f;
   for (long long row0 = begin; row0 < end; row0 += teams) {
     const long long row = row0 + mine;
-    float z[V][kVec], a[V][kVec], around[V][kVec];
+    float z[N][G], a[N][G], around[N][G];
     next.sum(z);
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      decode_vec<Out>(next_g[u], a[u]);
-      decode_vec<Sum>(next_s[u], around[u]);
+    for (int n = 0; n < N; ++n) {
+      Access<Out, G>::decode(next_g[n], a[n]);
+      Access<Sum, G>::decode(next_s[n], around[n]);
     }
     const float rstd = next_stats.y, shift = -next_stats.x * rstd;
     request(row + teams);
     float sums[2] = {0.f, 0.f};
     // beyond the width and the rows the gradients are zeros, and so is all that is added up
 #pragma unroll
-    for (int u = 0; u < V; ++u)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) {
-        z[u][c] = fmaf(z[u][c], rstd, shift);
-        dw[u][c] = fmaf(a[u][c], z[u][c], dw[u][c]);
-        db[u][c] += a[u][c];
-        a[u][c] *= w[u][c];
-        sums[0] += a[u][c];
-        sums[1] = fmaf(a[u][c], z[u][c], sums[1]);
+      for (int c = 0; c < G; ++c) {
+        z[n][c] = fmaf(z[n][c], rstd, shift);
+        dw[n][c] = fmaf(a[n][c], z[n][c], dw[n][c]);
+        db[n][c] += a[n][c];
+        a[n][c] *= w[n][c];
+        sums[0] += a[n][c];
+        sums[1] = fmaf(a[n][c], z[n][c], sums[1]);
       }
     team_sum(sums, g.team, s_slots, turn);
     if (row >= end) continue;
     const float m1 = sums[0] * inv, m2 = sums[1] * inv;
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-      if (width_live[u] == 0) continue;
-      const long long at = row * p.width + column[u];
+    for (int n = 0; n < N; ++n) {
+      if (!column.live[n]) continue;
+      const long long at = row * p.width + column.at[n];
 #pragma unroll
-      for (int c = 0; c < kVec; ++c) a[u][c] = fmaf(rstd, a[u][c] - m1 - z[u][c] * m2, around[u][c]);
-      if (p.grad_x != nullptr) store_vec<typename T::X>(element<typename T::X>(p.grad_x, at), width_live[u], a[u]);
+      for (int c = 0; c < G; ++c) a[n][c] = fmaf(rstd, a[n][c] - m1 - z[n][c] * m2, around[n][c]);
+      if (p.grad_x != nullptr) Access<typename T::X, G>::store(element<typename T::X>(p.grad_x, at), a[n]);
       if constexpr (T::kSum)
-        if (p.grad_residual != nullptr) store_vec<typename T::R>(element<typename T::R>(p.grad_residual, at), width_live[u], a[u]);
+        if (p.grad_residual != nullptr) Access<typename T::R, G>::store(element<typename T::R>(p.grad_residual, at), a[n]);
     }
   }
   if (p.grad_weight == nullptr && p.grad_bias == nullptr) return;
-  const int padded = (p.width + kVec - 1) / kVec * kVec;
-  float *part = static_cast<float *>(p.workspace) + (size_t)blockIdx.x * 2 * padded;
+  float *part = static_cast<float *>(p.workspace) + (size_t)blockIdx.x * 2 * p.width;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < V; ++u)
-      if (width_live[u] > 0)
+    for (int n = 0; n < N; ++n)
+      if (column.live[n])
 #pragma unroll
-        for (int c = 0; c < kVec; ++c) s_columns[(size_t)mine * padded + column[u] + c] = q == 0 ? dw[u][c] : db[u][c];
+        for (int c = 0; c < G; ++c) s_columns[(size_t)mine * p.width + column.at[n] + c] = q == 0 ? dw[n][c] : db[n][c];
     __syncthreads();
-    for (int c = threadIdx.x; c < padded; c += blockDim.x) {
+    for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
       float sum = 0.f;
-      for (int t = 0; t < teams; ++t) sum += s_columns[(size_t)t * padded + c];
-      part[(size_t)q * padded + c] = sum;
+      for (int t = 0; t < teams; ++t) sum += s_columns[(size_t)t * p.width + c];
+      part[(size_t)q * p.width + c] = sum;
     }
   }
 }
 
-// The workgroups' sums [blocks][2][padded width]: a workgroup takes 32 columns, 32 lanes each, four loads a lane under way; the lanes'
+// The workgroups' sums [blocks][2][width]: a workgroup takes 32 columns, 32 lanes each, four loads a lane under way; the lanes'
 // sums meet in LDS in their order.
 constexpr int kGradColumns = 32, kGradLanes = 32;
 __global__ void __launch_bounds__(kGradColumns * kGradLanes) add_norm_param_grad_kernel(const AddNormLaunch p, unsigned blocks) {
   __shared__ float s_part[kGradLanes][kGradColumns + 1];
-  const int padded = (p.width + kVec - 1) / kVec * kVec;
   const int c = threadIdx.x % kGradColumns, lane = threadIdx.x / kGradColumns, index = blockIdx.x * kGradColumns + c;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (index < 2 * padded) {
+  if (index < 2 * p.width) {
     const float *from = static_cast<const float *>(p.workspace) + index;
-    const size_t step = (size_t)2 * padded;
+    const size_t step = (size_t)2 * p.width;
     unsigned i = lane;
     for (; i + 3 * kGradLanes < blocks; i += 4 * kGradLanes)
 #pragma unroll
@@ -340,28 +331,32 @@ __global__ void __launch_bounds__(kGradColumns * kGradLanes) add_norm_param_grad
   }
   s_part[lane][c] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   __syncthreads();
-  if (lane != 0 || index >= 2 * padded) return;
-  const int column = index < padded ? index : index - padded;
-  void *to = index < padded ? p.grad_weight : p.grad_bias;
-  if (to == nullptr || column >= p.width) return;
-  float total[kVec] = {};
+  if (lane != 0 || index >= 2 * p.width) return;
+  void *to = index < p.width ? p.grad_weight : p.grad_bias;
+  if (to == nullptr) return;
+  float total[1] = {0.f};
 #pragma unroll
   for (int l = 0; l < kGradLanes; ++l) total[0] += s_part[l][c];
-  char *at = static_cast<char *>(to) + (long long)column * bytes_of(p.param_dtype);
-  if (p.param_dtype == F32::kCode) store_vec<F32>(at, 1, total);
-  else if (p.param_dtype == F16::kCode) store_vec<F16>(at, 1, total);
-  else store_vec<BF16>(at, 1, total);
+  char *at = static_cast<char *>(to) + (long long)(index < p.width ? index : index - p.width) * bytes_of(p.param_dtype);
+  if (p.param_dtype == F32::kCode) Access<F32, 1>::store(at, total);
+  else if (p.param_dtype == F16::kCode) Access<F16, 1>::store(at, total);
+  else Access<BF16, 1>::store(at, total);
 }
 
-// A lane has two vectors of rows of more than 64, so that a wave holds a row of up to 1024 channels and meets no barrier.
-int vectors_of(const AddNormLaunch &p) { return (p.width + kVec - 1) / kVec; }
-bool two_a_lane(const AddNormLaunch &p) { return vectors_of(p) > kWave; }
+// Whether every row of every tensor starts on 16 bytes and is whole vectors.
+bool in_vectors(const AddNormLaunch &p) {
+  auto fits = [](const void *base, long long bytes) { return reinterpret_cast<uintptr_t>(base) % 16 == 0 && bytes % 16 == 0; };
+  auto row_fits = [&](const NormRows &t) { return t.base == nullptr || fits(t.base, t.pitch * (t.dtype == F32::kCode ? 4 : 2)); };
+  return p.width % 8 == 0 && row_fits(p.x) && row_fits(p.residual) && fits(p.weight, 0) && fits(p.bias, 0) && fits(p.out, 0) && fits(p.sum, 0) &&
+         fits(p.grad_out, 0) && fits(p.grad_sum, 0) && fits(p.grad_x, 0) && fits(p.grad_residual, 0);
+}
+// Elements a lane: sixteen of rows of more than 512, so that a wave holds a row of up to 1024 channels and meets no barrier.
+int lane_elements(const AddNormLaunch &p) { return p.width > 512 ? 16 : 8; }
 // Parameters in registers pay over several rows; workgroups enough to fill the chip come first.
 Geometry geometry(const AddNormLaunch &p, long long most_blocks) {
   Geometry g;
-  const int vectors = (vectors_of(p) + two_a_lane(p)) / (two_a_lane(p) ? 2 : 1);
   g.team = 1;
-  while (g.team < vectors) g.team *= 2;
+  while (g.team * lane_elements(p) < p.width) g.team *= 2;
   g.threads = std::max(g.team, 64);
   if (g.team <= kWave && p.rows * g.team >= 256ll * 1024) g.threads = 256;
   const long long teams = g.threads / g.team, passes = (p.rows + teams - 1) / teams;
@@ -373,8 +368,7 @@ Geometry geometry(const AddNormLaunch &p, long long most_blocks) {
 Geometry forward_geometry(const AddNormLaunch &p) { return geometry(p, 4096); }
 Geometry backward_geometry(const AddNormLaunch &p) {
   // partial sums stay below 32 MB
-  const long long columns = (long long)vectors_of(p) * kVec;
-  return geometry(p, std::max<long long>(1, std::min<long long>(1024, (32ll << 20) / (8 * columns))));
+  return geometry(p, std::max<long long>(1, std::min<long long>(1024, (32ll << 20) / (8ll * p.width))));
 }
 
 template <typename T>
@@ -385,17 +379,17 @@ hipError_t run(const AddNormLaunch &p, hipStream_t stream, bool backward) {
     return hipGetLastError();
   }
   const Geometry g = backward_geometry(p);
-  const int padded = vectors_of(p) * kVec;
-  const size_t lds = (size_t)(g.threads / g.team) * padded * sizeof(float);
+  const size_t lds = (size_t)(g.threads / g.team) * p.width * sizeof(float);
   hipLaunchKernelGGL((add_norm_backward_kernel<T>), dim3(g.blocks), dim3(g.threads), lds, stream, p, g);
   if (hipError_t e = hipGetLastError()) return e;
   if (p.grad_weight == nullptr && p.grad_bias == nullptr) return hipSuccess;
-  hipLaunchKernelGGL(add_norm_param_grad_kernel, dim3((2 * padded + kGradColumns - 1) / kGradColumns), dim3(kGradColumns * kGradLanes), 0, stream, p, g.blocks);
+  hipLaunchKernelGGL(add_norm_param_grad_kernel, dim3((2 * p.width + kGradColumns - 1) / kGradColumns), dim3(kGradColumns * kGradLanes), 0, stream, p, g.blocks);
   return hipGetLastError();
 }
 template <typename X, typename R, bool WIDE>
 hipError_t with_types(const AddNormLaunch &p, hipStream_t stream, bool backward) {
-  return two_a_lane(p) ? run<Types<X, R, WIDE, 2>>(p, stream, backward) : run<Types<X, R, WIDE, 1>>(p, stream, backward);
+  if (in_vectors(p)) return lane_elements(p) == 8 ? run<Types<X, R, WIDE, 8, 1>>(p, stream, backward) : run<Types<X, R, WIDE, 8, 2>>(p, stream, backward);
+  return lane_elements(p) == 8 ? run<Types<X, R, WIDE, 1, 8>>(p, stream, backward) : run<Types<X, R, WIDE, 1, 16>>(p, stream, backward);
 }
 template <typename X>
 hipError_t with_residual(const AddNormLaunch &p, hipStream_t stream, bool backward) {
@@ -424,7 +418,7 @@ hipError_t launch(const AddNormLaunch &p, hipStream_t stream, bool backward) {
 
 size_t add_norm_backward_workspace_bytes(const AddNormLaunch &p) {
   if (p.grad_weight == nullptr && p.grad_bias == nullptr) return 0;
-  return (size_t)backward_geometry(p).blocks * 2 * vectors_of(p) * kVec * sizeof(float);
+  return (size_t)backward_geometry(p).blocks * 2 * p.width * sizeof(float);
 }
 hipError_t launch_add_norm_forward(const AddNormLaunch &p, hipStream_t stream) { return launch(p, stream, false); }
 hipError_t launch_add_norm_backward(const AddNormLaunch &p, hipStream_t stream) { return launch(p, stream, true); }

@@ -427,15 +427,31 @@ NormInputs norm_inputs(Args &a) {
   return in;
 }
 
-// add_layer_norm(input, residual, weight, bias, eps, wide, want_sum): the result or (result, sum), or None as above
+// Whether the kernels take a call as it is: rows of a length and of types that they know, all on one GPU.
+bool norm_takes(const NormInputs &a) {
+  if (!a.x.is_cuda() || a.x.dim() < 1 || a.x.size(-1) < 1 || a.x.size(-1) > kMaxNormWidth) return false;
+  at::ScalarType half = at::kFloat;
+  for (const Tensor *t : {&a.x, &a.residual, &a.weight, &a.bias}) {
+    if (!t->defined()) continue;
+    const at::ScalarType type = t->scalar_type();
+    if (t->device() != a.x.device() || (type != at::kFloat && type != at::kHalf && type != at::kBFloat16)) return false;
+    if (type != at::kFloat && half != at::kFloat && type != half) return false;
+    if (type != at::kFloat) half = type;
+    if (!plain(*t)) return false;
+  }
+  if (a.residual.defined() && a.residual.sizes() != a.x.sizes()) return false;
+  for (const Tensor *t : {&a.weight, &a.bias})
+    if (t->defined() && (t->dim() != 1 || t->size(0) != a.x.size(-1))) return false;
+  return !a.weight.defined() || !a.bias.defined() || a.weight.scalar_type() == a.bias.scalar_type();
+}
+
+// add_layer_norm(input, residual, weight, bias, eps, wide, want_sum): the result or (result, sum), or None where it is not taken
 PyObject *py_add_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a("add_layer_norm", args, n, 7);
   const NormInputs in = norm_inputs(a);
   const bool want_sum = a.integer() != 0;
-  if (observed()) Py_RETURN_NONE;
-  for (const Tensor *t : {&in.x, &in.residual, &in.weight, &in.bias})
-    if (t->defined() && !plain(*t)) Py_RETURN_NONE;
+  if (observed() || !norm_takes(in)) Py_RETURN_NONE;
   NormOutputs o;
   {
     pybind11::gil_scoped_release no_gil;

@@ -58,9 +58,13 @@ def add_layer_norm(x, residual, norm, return_sum=False):
     """``norm(x + residual)`` for an ``nn.LayerNorm`` over the last axis; ``residual`` of x's shape, or None.  The result has the
     wider type of the two, float32 under autocast as torch's own layer norm there.  With ``return_sum`` also the sum, in the wider type:
     ``(result, x + residual)``, the stream of a pre-norm network."""
+    weight, bias, wide = norm.weight, norm.bias, torch.is_autocast_enabled()
+    if weight is not None or tuple(norm.normalized_shape) == (x.shape[-1],):      # (the weight says as much)
+        output = _native.add_layer_norm(x, residual, weight, bias, norm.eps, wide, return_sum)
+        if output is not None:
+            return output
     if not _fusable(x, residual, norm):
         total = x if residual is None else x + residual
         out = norm(total)
         return (out, total) if return_sum else out
-    wide = torch.is_autocast_enabled()
-    return AddLayerNormFunction.apply(x, residual, norm.weight, norm.bias, norm.eps, wide, bool(return_sum))
+    return AddLayerNormFunction.apply(x, residual, weight, bias, norm.eps, wide, bool(return_sum))
