@@ -142,18 +142,46 @@ template <typename S>
 __device__ __forceinline__ u32x4 fragment(const char *tensor, int block, int slice, int lane) {
   return *reinterpret_cast<const u32x4 *>(tensor + slice * S::RT * 64 + block * 1024 + fragment_at(lane & 15, lane >> 4));
 }
-// acc[d][f] += rows 16 block .. + 31 of the tensor, turned, times the weights in p[0], p[1]
+// Weights of 32 rows as the second operand of a product; 16-bit types round them, rest() is what that took.
 template <typename S>
-__device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF], const char *tensor, int block, const f32x4 (&p)[2][S::CF], int lane) {
+struct Weights {
+  typedef typename S::Tag Tag;
+  static constexpr bool kHalf = Tag::kBytes == 2;
+  u32x4 half[kHalf ? S::CF : 1];
+  f32x4 full[kHalf ? 1 : 2][kHalf ? 1 : S::CF];
+  __device__ __forceinline__ explicit Weights(const f32x4 (&p)[2][S::CF]) {
+#pragma unroll
+    for (int f = 0; f < S::CF; ++f) {
+      if constexpr (kHalf) {
+        const float v[8] = {p[0][f].x, p[0][f].y, p[0][f].z, p[0][f].w, p[1][f].x, p[1][f].y, p[1][f].z, p[1][f].w};
+        half[f] = Pack<Tag, 8>::encode(v);
+      } else {
+        full[0][f] = p[0][f];
+        full[1][f] = p[1][f];
+      }
+    }
+  }
+  __device__ __forceinline__ Weights rest(const f32x4 (&p)[2][S::CF]) const {
+    f32x4 left[2][S::CF];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const uint32_t pair = half[f][h * 2 + r / 2];
+          left[h][f][r] = -plus_half<Tag, 0>(pair, -p[h][f][r]);
+          left[h][f][r + 1] = -plus_half<Tag, 1>(pair, -p[h][f][r + 1]);
+        }
+    return Weights(left);
+  }
+};
+// acc[d][f] += rows 16 block .. + 31 of the tensor, turned, times the weights, and where SETS is 2 times more weights
+template <typename S, int SETS = 1>
+__device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF], const char *tensor, int block, const Weights<S> &w, const Weights<S> &more, int lane) {
   typedef typename S::Tag Tag;
   const int g = lane >> 4, c = lane & 15;
   if constexpr (Tag::kBytes == 2) {
-    u32x4 w[S::CF];
-#pragma unroll
-    for (int f = 0; f < S::CF; ++f) {
-      const float v[8] = {p[0][f].x, p[0][f].y, p[0][f].z, p[0][f].w, p[1][f].x, p[1][f].y, p[1][f].z, p[1][f].w};
-      w[f] = Pack<Tag, 8>::encode(v);
-    }
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) {
       const char *at = tensor + d / 2 * S::RT * 64 + block * 1024 + (4 * g + (c >> 2)) * 64 + (((d & 1) * 2 + ((c & 3) >> 1)) ^ turned_by(g)) * 16 + (c & 1) * 8;
@@ -162,7 +190,10 @@ __device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF]
       const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
       const u32x4 turned = {a.x, a.y, b.x, b.y};
 #pragma unroll
-      for (int f = 0; f < S::CF; ++f) acc[d][f] = mfma_64_bytes<Tag>(turned, w[f], acc[d][f]);
+      for (int f = 0; f < S::CF; ++f) {
+        acc[d][f] = mfma_64_bytes<Tag>(turned, w.half[f], acc[d][f]);
+        if constexpr (SETS == 2) acc[d][f] = mfma_64_bytes<Tag>(turned, more.half[f], acc[d][f]);
+      }
     }
   } else {
 #pragma unroll
@@ -174,10 +205,15 @@ __device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF]
         for (int r = 0; r < 4; ++r) {
           const float a = *reinterpret_cast<const float *>(at + r * 64);
 #pragma unroll
-          for (int f = 0; f < S::CF; ++f) acc[d][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, p[half][f][r], acc[d][f], 0, 0, 0);
+          for (int f = 0; f < S::CF; ++f) acc[d][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w.full[half][f][r], acc[d][f], 0, 0, 0);
         }
       }
   }
+}
+template <typename S>
+__device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF], const char *tensor, int block, const f32x4 (&p)[2][S::CF], int lane) {
+  const Weights<S> w(p);
+  add_product<S>(acc, tensor, block, w, w, lane);
 }
 
 // A column's operand, straight from memory: the second operand of the score products.
@@ -505,10 +541,11 @@ __device__ __forceinline__ f32x4 rounded_off(f32x4 v) {
 // ---------------------------------------------------------------- forward
 struct Split {
   int tiles, chunks, chunk_rows;      // column tiles of a head; parts of the rows, a whole number of tiles each
-  float *part, *stats;                // [chunk][batch][query][head][width], [..][4]: unnormalised sums; maximum, sum, exact sum
+  float *part, *stats;                // [chunk][batch][query][head][width], [..][2]: unnormalised sums; maximum and sum
 };
 
-template <typename S>
+// TRAIN: a backward follows (16-bit types; fp32 ones have nothing to round).
+template <typename S, bool TRAIN>
 __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_kernel(const AttnLaunch p, const Split split) {
   typedef typename S::Tag Tag;
   extern __shared__ __align__(16) char lds[];
@@ -543,15 +580,14 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
   }
   const ColumnRange range = masked ? column_range<false>(q_segments, column0, p.nq, S::kColumns, lane) : ColumnRange{};
 
-  // total: sums of the weights as the product takes them, rounded, which divide the result; exact: of the weights themselves, for the
-  // logarithm from which the backward forms them again
+  // total: sums of the weights as the product takes them.  In 16-bit types that is rounded; where a backward follows, what rounding took
+  // goes through the products as well: delta, and the logarithm from which the weights are formed again, then belong to the weights
+  // themselves (with delta of rounded ones dQ was off by 1.5 of its own roundings, with those of 1.4).
   f32x4 acc[S::kWidthBlocks][S::CF], total[S::CF];
-  float top[S::CF], exact[S::CF];
-  const bool train = Tag::kBytes == 2 && p.lse != nullptr;
+  float top[S::CF];
 #pragma unroll
   for (int f = 0; f < S::CF; ++f) {
     top[f] = -kInf;
-    exact[f] = 0.f;
     total[f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -624,7 +660,6 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
 #pragma unroll
         for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] *= keep;
         total[f] *= keep;
-        exact[f] *= keep;
       }
 #pragma unroll
     for (int f = 0; f < S::CF; ++f) {
@@ -634,25 +669,35 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[n][f][r] = __builtin_amdgcn_exp2f(fmaf(s[n][f][r], factor, off));
     }
-    if (Tag::kBytes == 4 || train)
+    if constexpr (Tag::kBytes == 4)
 #pragma unroll
       for (int f = 0; f < S::CF; ++f)
 #pragma unroll
-        for (int n = 0; n < S::kRowBlocks; ++n) exact[f] += (s[n][f].x + s[n][f].y) + (s[n][f].z + s[n][f].w);
+        for (int n = 0; n < S::kRowBlocks; ++n) total[f] += s[n][f];
 #pragma unroll
     for (int n = 0; n < S::kRowBlocks; n += 2) {
-      f32x4 w[2][S::CF];
+      f32x4 p32[2][S::CF];
 #pragma unroll
       for (int f = 0; f < S::CF; ++f) {
-        w[0][f] = s[n][f];
-        w[1][f] = s[n + 1][f];
-        if constexpr (Tag::kBytes == 2) {      // of the weights as the product takes them
-          constexpr uint32_t one = Tag::kCode == F16::kCode ? 0x3c003c00u : 0x3f803f80u;
-          const float v[8] = {w[0][f].x, w[0][f].y, w[0][f].z, w[0][f].w, w[1][f].x, w[1][f].y, w[1][f].z, w[1][f].w};
-          total[f] = mfma_64_bytes<Tag>(u32x4{one, one, one, one}, Pack<Tag, 8>::encode(v), total[f]);
-        }
+        p32[0][f] = s[n][f];
+        p32[1][f] = s[n + 1][f];
       }
-      add_product<S>(acc, tile + S::kTensorBytes, block0 + n, w, lane);
+      const Weights<S> w(p32);
+      auto count = [&](const Weights<S> &v) {
+        constexpr uint32_t one = Tag::kCode == F16::kCode ? 0x3c003c00u : 0x3f803f80u;
+#pragma unroll
+        for (int f = 0; f < S::CF; ++f) total[f] = mfma_64_bytes<Tag>(u32x4{one, one, one, one}, v.half[f], total[f]);
+      };
+      if constexpr (Tag::kBytes == 2) {
+        count(w);
+      }
+      if constexpr (TRAIN) {
+        const Weights<S> left = w.rest(p32);
+        count(left);
+        add_product<S, 2>(acc, tile + S::kTensorBytes, block0 + n, w, left, lane);
+      } else {
+        add_product<S>(acc, tile + S::kTensorBytes, block0 + n, w, w, lane);
+      }
     }
   };
   walk_tiles<S, false>(k_segments, masked, range, first, last, lds, s_flags, wave, lane, request, put, work);
@@ -660,21 +705,20 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
   float sum[S::CF];
 #pragma unroll
   for (int f = 0; f < S::CF; ++f) {
-    exact[f] = column_sum(exact[f]);
-    sum[f] = Tag::kBytes == 4 ? exact[f] : total[f].x;
+    sum[f] = Tag::kBytes == 4 ? column_sum((total[f].x + total[f].y) + (total[f].z + total[f].w)) : total[f].x;
     if (segment[f] < 0) {      // sees nothing
-      sum[f] = exact[f] = 0.f;
+      sum[f] = 0.f;
       top[f] = -kInf;
 #pragma unroll
       for (int d = 0; d < S::kWidthBlocks; ++d) acc[d][f] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
   if constexpr (S::RW > 1) {
-    f32x4 *s_stats = reinterpret_cast<f32x4 *>(lds + S::kMergeStats);
+    f32x2 *s_stats = reinterpret_cast<f32x2 *>(lds + S::kMergeStats);
     auto slot = [&](int w, int f) { return ((w * S::kColumnWaves + column_wave) * S::CF + f) * 16 + c; };
 #pragma unroll
     for (int f = 0; f < S::CF; ++f)
-      if (g == 0) s_stats[slot(row_wave, f)] = f32x4{top[f], sum[f], exact[f], 0.f};
+      if (g == 0) s_stats[slot(row_wave, f)] = f32x2{top[f], sum[f]};
     __syncthreads();
 #pragma unroll
     for (int f = 0; f < S::CF; ++f) {
@@ -683,14 +727,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
 #pragma unroll
       for (int w = 0; w < S::RW; ++w) now = fmaxf(now, s_stats[slot(w, f)].x);
       const float base = now == -kInf ? 0.f : now;
-      sum[f] = exact[f] = 0.f;
+      sum[f] = 0.f;
 #pragma unroll
-      for (int w = 0; w < S::RW; ++w) {
-        const f32x4 of = s_stats[slot(w, f)];
-        const float keep = __builtin_amdgcn_exp2f(of.x - base);
-        sum[f] = fmaf(of.y, keep, sum[f]);
-        exact[f] = fmaf(of.z, keep, exact[f]);
-      }
+      for (int w = 0; w < S::RW; ++w) sum[f] = fmaf(s_stats[slot(w, f)].y, __builtin_amdgcn_exp2f(s_stats[slot(w, f)].x - base), sum[f]);
       const float keep = __builtin_amdgcn_exp2f(was - base);
       top[f] = now;
 #pragma unroll
@@ -719,9 +758,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
       }
     }
     if (g != 0 || row_wave != 0) continue;
-    if (split_rows) reinterpret_cast<f32x4 *>(split.stats)[part_row] = f32x4{top[f], sum[f], exact[f], 0.f};
+    if (split_rows) reinterpret_cast<f32x2 *>(split.stats)[part_row] = f32x2{top[f], sum[f]};
     else if (p.lse != nullptr)
-      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = exact[f] == 0.f ? kInf : top[f] - kForwardShift<Tag> + __builtin_amdgcn_logf(exact[f]);
+      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = sum[f] == 0.f ? kInf : top[f] - kForwardShift<Tag> + __builtin_amdgcn_logf(sum[f]);
   }
 }
 
@@ -731,26 +770,24 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnLaunc
   const int lane = threadIdx.x % kWave, teams = kWave / lanes, team = lane / lanes, column = lane % lanes * 4;
   const long long rows = (long long)p.batch * p.nq * p.heads, row = (long long)blockIdx.x * kJoinWaves + threadIdx.x / kWave;
   if (row >= rows) return;
-  const f32x4 *stats = reinterpret_cast<const f32x4 *>(split.stats);
+  const f32x2 *stats = reinterpret_cast<const f32x2 *>(split.stats);
   float top = -kInf;
   for (int k = lane; k < split.chunks; k += kWave) top = fmaxf(top, stats[k * rows + row].x);
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
   const float base = top == -kInf ? 0.f : top;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f, exact = 0.f;
+  float sum = 0.f;
 #pragma unroll 4
   for (int k = team; k < split.chunks; k += teams) {
-    const f32x4 s = stats[k * rows + row];
+    const f32x2 s = stats[k * rows + row];
     const float w = __builtin_amdgcn_exp2f(s.x - base);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (column < p.width) v = *reinterpret_cast<const f32x4 *>(split.part + (k * rows + row) * p.width + column);
     sum = fmaf(w, s.y, sum);
-    exact = fmaf(w, s.z, exact);
     acc += v * w;
   }
   for (int o = lanes; o < kWave; o <<= 1) {
     sum += __shfl_xor(sum, o, kWave);
-    exact += __shfl_xor(exact, o, kWave);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o, kWave);
   }
@@ -760,7 +797,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnLaunc
   if (p.out_rest != nullptr) store4<Tag>(p.out_rest, row * p.width + column, rounded_off<Tag>(acc));
   if (p.lse != nullptr && column == 0) {
     const long long head = row % p.heads, i = row / p.heads % p.nq, b = row / p.heads / p.nq;
-    p.lse[(b * p.heads + head) * p.nq + i] = exact == 0.f ? kInf : top - kForwardShift<Tag> + __builtin_amdgcn_logf(exact);
+    p.lse[(b * p.heads + head) * p.nq + i] = sum == 0.f ? kInf : top - kForwardShift<Tag> + __builtin_amdgcn_logf(sum);
   }
 }
 
@@ -1304,7 +1341,7 @@ size_t part_bytes(const AttnLaunch &p, const Split &s) {
   return s.chunks > 1 ? padded((size_t)s.chunks * p.batch * p.nq * p.heads * p.width * sizeof(float)) : 0;
 }
 size_t forward_bytes(const AttnLaunch &p, const Split &s) {
-  return s.chunks > 1 ? part_bytes(p, s) + padded((size_t)s.chunks * p.batch * p.nq * p.heads * 4 * sizeof(float)) : 0;
+  return s.chunks > 1 ? part_bytes(p, s) + padded((size_t)s.chunks * p.batch * p.nq * p.heads * 2 * sizeof(float)) : 0;
 }
 
 template <typename S>
@@ -1318,7 +1355,9 @@ hipError_t forward_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
   s.part = static_cast<float *>(p.workspace);
   s.stats = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + part_bytes(p, s));
   const long long blocks = (long long)p.batch * p.heads * s.tiles * s.chunks;
-  if (hipError_t e = run<S>(attn_forward_kernel<S>, blocks, stream, p, s)) return e;
+  constexpr bool half = Tag::kBytes == 2;
+  const bool train = half && p.lse != nullptr;
+  if (hipError_t e = train ? run<S>(attn_forward_kernel<S, half>, blocks, stream, p, s) : run<S>(attn_forward_kernel<S, false>, blocks, stream, p, s)) return e;
   if (s.chunks == 1) return hipSuccess;
   hipLaunchKernelGGL((attn_join_kernel<Tag>), dim3((unsigned)ceil_div((long long)p.batch * p.nq * p.heads, kJoinWaves)), dim3(kJoinThreads), 0, stream, p, s,
                      row_lanes(p));
