@@ -1,5 +1,7 @@
 // What stands between the sampling layers of a deformable decoder: attention among queries and the normalised sum.  Checks, dense
 // rows where the kernels need them, allocation and autograd nodes.
+#include <cmath>
+
 #include "../add_norm.hpp"
 #include "../query_attention.hpp"
 #include "layers.hpp"
@@ -8,6 +10,7 @@ namespace dcn::binding {
 namespace {
 
 constexpr int64_t kIntMax = 0x7fffffff;
+constexpr float kFloatMax = 3.402823466e38f;
 
 // ---------------------------------------------------------------- attention among queries
 struct AttnInputs {
@@ -51,7 +54,8 @@ AttnShape attn_check(const AttnInputs &a) {
   // rows are counted in 32 bits by the kernels
   if (s.nq > (1 << 30) || s.nk > (1 << 30)) raise_runtime("sequences of more than 2^30 tokens");
   if (s.batch * s.nq * s.heads > kIntMax || s.batch * s.nk * s.kv_heads > kIntMax) raise_runtime("more than 2^31 - 1 rows of queries or keys");
-  if (!(a.scale == a.scale) || !(a.cap >= 0.f) || a.cap > 3e38f) raise_runtime("cap must be zero (none) or positive and finite, scale a number");
+  if (!(std::fabs(a.scale) < kFloatMax)) raise_runtime("scale must be finite");
+  if (a.cap != 0.f && !(a.cap >= 1e-30f && a.cap <= 1e30f)) raise_runtime("cap must be zero (none) or between 1e-30 and 1e30");
   if (a.q_segments.defined()) {
     check_beside(a.q_segments, "segments", a.q, at::kInt, {s.batch, s.nq});
     if (!a.k_segments.defined()) raise_runtime("segments without key_segments");

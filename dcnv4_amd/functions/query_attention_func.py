@@ -60,8 +60,11 @@ def query_attention(query, key, value, *, scale=None, cap=0.0, segments=None, ke
     (M,) float32.  Gradients reach query, key, value and slopes.  Under autocast the first three are cast to its type.
     Returns (N, Lq, M, D)."""
     for points in (positions, key_positions):
-        if points is not None and points.requires_grad:
+        if points is not None and points.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("query_attention has no gradient for positions: detach them")
+    cap = float(cap or 0.0)
+    if cap != 0.0 and not 1e-30 <= cap <= 1e30:      # (what is smaller is zero as a float)
+        raise RuntimeError("cap must be zero (none) or between 1e-30 and 1e30")
     if torch.is_autocast_enabled() and query.is_cuda:
         dtype = torch.get_autocast_dtype("cuda")
         query, key, value = (t.to(dtype) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (query, key, value))
@@ -71,5 +74,4 @@ def query_attention(query, key, value, *, scale=None, cap=0.0, segments=None, ke
         key_positions = positions
     if scale is None:
         scale = query.shape[-1] ** -0.5 if query.dim() and query.shape[-1] else 1.0
-    return QueryAttentionFunction.apply(query, key, value, segments, key_segments, positions, key_positions, slopes, float(scale),
-                                        float(cap or 0.0))
+    return QueryAttentionFunction.apply(query, key, value, segments, key_segments, positions, key_positions, slopes, float(scale), cap)

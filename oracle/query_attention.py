@@ -1,4 +1,4 @@
-"""Dense attention with capped scores, a bias by distance and segment masks, in float64 on the CPU, and how far a kernel may be
+"""Dense attention with capped scores, a bias by distance and segment masks, in float64, and how far a kernel may be
 from it: every result comes with the size of what was summed into it, for tolerances that count roundings.
 
   x = scale q k^T,  s = cap tanh(x / cap) - slope |p_q - p_k|,  P = softmax(s) over visible keys,  out = P v
@@ -17,7 +17,7 @@ def visible(q_segments, k_segments):
 
 
 def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segments=None, q_points=None, k_points=None, slopes=None,
-              unit=2.0 ** -53, tiny=0.0):
+              unit=2.0 ** -53, tiny=0.0, device="cpu"):
     """Results in float64 and their tolerances for tensors of a type with rounding unit ``unit`` (half a step, relative) and smallest
     rounding ``tiny`` (half the step of its subnormals): dict name -> (value, tolerance).
 
@@ -26,11 +26,12 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
     e = (width + 8) 2^-24 times the sum of their sizes (cap, slope times distance and the score itself counted in), a weight by 2 e and
     the sum over the keys, relatively.  The scale of dS in fp16 keeps it below 2^15 by width max|g| max|v|, so that tiny weighs 2^-15 of
     twice that.  Sizes are floats of all heads, key heads already spread over the heads that share them."""
-    q, k, v = (t.detach().cpu().double() for t in (q, k, v))
+    to = lambda t: t.detach().to(device).double()
+    q, k, v = to(q), to(k), to(v)
     n, lq, m, d = q.shape
     lk, share = k.shape[1], m // k.shape[2]
     scale = d ** -0.5 if scale is None else scale
-    spread = torch.arange(m) // share
+    spread = torch.arange(m, device=device) // share
     qh, kh, vh = q.permute(0, 2, 1, 3), k[:, :, spread].permute(0, 2, 1, 3), v[:, :, spread].permute(0, 2, 1, 3)
     x = scale * (qh @ kh.transpose(-1, -2))
     size = abs(scale) * (qh.abs() @ kh.abs().transpose(-1, -2))
@@ -40,20 +41,20 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
         th = torch.tanh(x / cap)
         s = cap * th
         size = size + cap
-    dist = torch.zeros(n, 1, lq, lk, dtype=torch.float64)
+    dist = torch.zeros(n, 1, lq, lk, dtype=torch.float64, device=device)
     if slopes is not None:
-        pq, pk = q_points.detach().cpu().double(), k_points.detach().cpu().double()
+        pq, pk = to(q_points), to(k_points)
         dist = (pq[:, :, None] - pk[:, None]).pow(2).sum(-1).sqrt()[:, None]
-        bias = slopes.detach().cpu().double().view(1, m, 1, 1) * dist
+        bias = to(slopes).view(1, m, 1, 1) * dist
         s = s - bias
         size = size + bias.abs()
-    see = torch.ones(n, 1, lq, lk, dtype=torch.bool)
+    see = torch.ones(n, 1, lq, lk, dtype=torch.bool, device=device)
     if k_segments is not None:
-        mine = torch.zeros(n, lq, dtype=torch.int32) if q_segments is None else q_segments.cpu()
-        see = visible(mine, k_segments.cpu())[:, None]
+        mine = torch.zeros(n, lq, dtype=torch.int32, device=device) if q_segments is None else q_segments.to(device)
+        see = visible(mine, k_segments.to(device))[:, None]
     see = see.expand_as(s)
     s = torch.where(see, s, -math.inf)
-    top = s.amax(-1, keepdim=True) if lk else torch.zeros(n, m, lq, 1, dtype=torch.float64)
+    top = s.amax(-1, keepdim=True) if lk else torch.zeros(n, m, lq, 1, dtype=torch.float64, device=device)
     p = torch.where(see, torch.exp(s - torch.where(torch.isfinite(top), top, 0.0)), 0.0)
     total = p.sum(-1, keepdim=True)
     p = p / torch.where(total > 0, total, 1.0)
@@ -69,7 +70,7 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
     found = {"out": (back(out), back(unit * out.abs() + (2 * unit + error) * (p @ vh.abs()) + tiny * (see.double() @ vh.abs())) + tiny)}
     if grad is None:
         return found
-    g = clean(grad.detach().cpu().double().permute(0, 2, 1, 3))
+    g = clean(to(grad).permute(0, 2, 1, 3))
     dp = g @ vh.transpose(-1, -2)
     delta = (p * dp).sum(-1, keepdim=True)
     ds = p * (dp - delta)

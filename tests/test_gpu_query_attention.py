@@ -1,4 +1,4 @@
-"""query_attention against float64 on the CPU (oracle/query_attention.py, which also says how far roundings can take a result), at the
+"""query_attention against float64 (oracle/query_attention.py, which also says how far roundings can take a result), at the
 lengths, widths, masks and layouts where a tiled kernel can go wrong."""
 import pytest
 import torch
@@ -71,14 +71,14 @@ def leaves(t):
 
 def close(got, want, what):
     value, tolerance = want
-    got = got.detach().cpu().double()
+    got = got.detach().to(value.device).double()
     assert got.shape == value.shape, (what, got.shape, value.shape)
     assert torch.isfinite(got).all(), f"{what}: not finite"
     beyond = (got - value).abs() - tolerance
     assert beyond.numel() == 0 or beyond.max() <= 0, f"{what}: {beyond.max():.3e} beyond tolerance, error {(got - value).abs().max():.3e}"
 
 
-def check(t, train=True, **kw):
+def check(t, train=True, device="cpu", **kw):
     dtype = t["q"].dtype
     gpu = on_gpu(t)
     wanted = leaves(gpu) if train else []
@@ -86,7 +86,7 @@ def check(t, train=True, **kw):
     assert out.dtype == dtype and out.is_contiguous()
     want = oracle_attention.attention(t["q"], t["k"], t["v"], t["grad"] if train else None, q_segments=t["q_segments"],
                                       k_segments=t["k_segments"], q_points=t["q_points"], k_points=t["k_points"], slopes=t["slopes"],
-                                      unit=UNIT[dtype], tiny=TINY[dtype], **kw)
+                                      unit=UNIT[dtype], tiny=TINY[dtype], device=device, **kw)
     close(out, want["out"], "out")
     if train:
         for name, got in zip(("grad_query", "grad_key", "grad_value", "grad_slopes"), torch.autograd.grad(out, wanted, gpu["grad"])):
@@ -142,6 +142,63 @@ def test_scores_that_grow_along_the_row(dtype):
     t["k"] = (t["k"].float() * 0.05 + torch.linspace(-1, 1, 700).view(1, -1, 1, 1)).to(dtype)
     t["q"] = (t["q"].float() * 0.05 + torch.linspace(-6, 6, 40).view(1, -1, 1, 1)).to(dtype)
     check(t)
+
+
+# heads and queries for every number of columns a workgroup takes, forward and backward, with and without masks
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("n,m,lq,mask", [(1, 2, 200, "none"), (1, 8, 1030, "random"), (1, 16, 1030, "none"), (2, 16, 1030, "none"), (2, 16, 600, "documents")])
+@pytest.mark.parametrize("width", (32, 64, 128))
+def test_every_shape_of_workgroup(width, n, m, lq, mask, dtype):
+    check(inputs(n, lq, lq, m, m, width, dtype, mask=mask, seed=width + m), device="cuda")
+
+
+@pytest.mark.parametrize("width", (32, 64))
+def test_many_heads_with_masks(width):
+    check(inputs(8, 1030, 1030, 16, 16, width, F16, mask="prefix", seed=width), device="cuda")
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("scale", (-0.4, 0.0, 1e-12, 3.0))
+def test_scales(scale, dtype):
+    t = inputs(1, 90, 130, 2, 2, 16, dtype, mask="random", seed=31, spread=0.7)
+    check(t, scale=scale)
+    check(t, scale=scale, cap=5.0)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+def test_distances_of_any_size_and_slope(dtype):
+    t = inputs(1, 70, 90, 6, 3, 16, dtype, mask="padding", distance=True, seed=32)
+    t["slopes"] = torch.tensor([0.0, 1e-30, -3.0, 40.0, 1e-4, -1e-20])
+    check(t)
+    t["q_points"], t["k_points"] = t["q_points"] * 1000, t["k_points"] * 1000      # pixels
+    t["slopes"] = t["slopes"] * 1e-3
+    check(t, cap=6.0)
+
+
+def test_a_memory_whose_offsets_pass_32_bits():
+    # 4.3e9 elements; of 17 million keys the last hundred are seen, and some in between
+    n = (1 << 24) + 77
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    k = torch.empty(1, n, 8, 32, dtype=F16, device="cuda").normal_(generator=gen)
+    v = torch.empty_like(k).normal_(generator=gen)
+    q = torch.randn(1, 3, 8, 32, generator=gen, device="cuda").to(F16)
+    ids = torch.full((1, n), -1, dtype=torch.int32, device="cuda")
+    seen = torch.cat((torch.arange(n // 2, n // 2 + 50, device="cuda"), torch.arange(n - 100, n, device="cuda")))
+    ids[:, seen] = 0
+    from dcnv4_amd.functions import query_attention
+    few = [x[:, seen].contiguous().requires_grad_() for x in (k, v)]
+    out = query_attention(q, few[0], few[1])
+    whole = query_attention(q, k, v, key_segments=ids)
+    # the same weights, added up in another order and from another maximum: a rounding of each weight and of the result
+    assert (whole.float() - out.float()).abs().max() <= 4 * UNIT[F16] * v[:, seen].float().abs().max()
+    grad = torch.randn(1, 3, 8, 32, generator=gen, device="cuda").to(F16)
+    want = torch.autograd.grad(out, few, grad)
+    k.requires_grad_()
+    v.requires_grad_()
+    got = torch.autograd.grad(query_attention(q, k, v, key_segments=ids), (k, v), grad)
+    for a, b in zip(got, want):
+        assert (a[:, seen].float() - b.float()).abs().max() <= 8 * UNIT[F16] * b.float().abs().max()
+        assert torch.count_nonzero(a) == torch.count_nonzero(a[:, seen])
 
 
 @pytest.mark.parametrize("dtype", (F16, BF16), ids=IDS.get)
@@ -407,5 +464,8 @@ def test_refusals():
     refused("slopes", positions=z(2, 5, 2, dtype=F32), key_positions=z(2, 7, 2, dtype=F32), slopes=z(2, dtype=F32))
     refused("no gradient for positions", positions=z(2, 5, 2, dtype=F32).requires_grad_(), key_positions=z(2, 7, 2, dtype=F32), slopes=z(4, dtype=F32))
     refused("cap", cap=-1.0)
+    refused("cap", cap=1e-60)
+    refused("scale", scale=float("inf"))
+    refused("scale", scale=float("nan"))
     refused("cap", cap=float("inf"))
     refused("cap", cap=float("nan"))
