@@ -36,4 +36,14 @@ hipError_t launch_attn_forward(int dtype, const AttnLaunch &p, hipStream_t strea
 // Wants out, out_rest and lse of the forward.
 hipError_t launch_attn_backward(int dtype, const AttnLaunch &p, hipStream_t stream);
 
+// A type's own (query_attention_*.hip): the launch, or where `bytes` is not null the scratch it wants and no launch.
+hipError_t attn_forward_fp32(const AttnLaunch &p, hipStream_t stream, size_t *bytes);
+hipError_t attn_forward_fp16(const AttnLaunch &p, hipStream_t stream, size_t *bytes);
+hipError_t attn_forward_bf16(const AttnLaunch &p, hipStream_t stream, size_t *bytes);
+hipError_t attn_backward_fp32(const AttnLaunch &p, hipStream_t stream, size_t *bytes);
+hipError_t attn_backward_fp16(const AttnLaunch &p, hipStream_t stream, size_t *bytes);
+hipError_t attn_backward_bf16(const AttnLaunch &p, hipStream_t stream, size_t *bytes);
+// grad[head] = sum over batch and parts of part[batch][heads][parts]
+hipError_t launch_slope_grad(const float *part, float *grad, int batch, int heads, int parts, hipStream_t stream);
+
 }  // namespace dcn
