@@ -960,7 +960,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
     }
   };
   auto work = [&](const char *tile, bool every) {
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < S::kRowBlocks; n += 2) {
       const int block = row_wave * S::kRowBlocks + n;
       f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
@@ -1159,7 +1159,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
       }
     };
     auto work = [&](const char *tile, bool every) {
-#pragma unroll
+#pragma unroll 1
       for (int n = 0; n < S::kRowBlocks; n += 2) {
         const int block = row_wave * S::kRowBlocks + n;
         f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
