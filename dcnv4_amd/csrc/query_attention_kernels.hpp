@@ -53,9 +53,10 @@ __device__ __forceinline__ float column_sum(float v) {
 
 // A kernel's shape.  W: the width, zeros behind the tensors' own; RT: rows of a tile; RW: waves that share the columns and divide
 // a tile's rows, the others divide the columns; CF: sixteens of columns a wave; WAVES: of a workgroup.
-template <typename Tag_, int W_, int RT_, int RW_, int CF_, int WAVES_>
+template <typename Tag_, bool PLAIN_, int W_, int RT_, int RW_, int CF_, int WAVES_>
 struct Shape {
   typedef Tag_ Tag;
+  static constexpr bool kPlain = PLAIN_;
   static constexpr int W = W_, RT = RT_, RW = RW_, CF = CF_, kWaves = WAVES_, kThreads = kWaves * kWave;
   static constexpr int kSlices = W * Tag::kBytes / 64, kWidthBlocks = W / 16;
   static constexpr int kColumnWaves = kWaves / RW, kColumns = 16 * CF * kColumnWaves;
@@ -244,6 +245,7 @@ __device__ __forceinline__ float dot_16_bytes(u32x4 a, u32x4 b, float sum) {
 // ---------------------------------------------------------------- scores
 // Scores go into exp2, so they are in units of its exponent.  Without cap and distance that is one factor, which rides along where
 // the maximum is taken off.
+template <bool PLAIN>
 struct Scores {
   float tanh_scale, factor, slope;
   bool bent, apart, scaled;      // there is a cap; a distance; neither, but a factor that cannot ride along
@@ -251,9 +253,17 @@ struct Scores {
     tanh_scale = bent ? p.scale / p.cap : 0.f;
     factor = (bent ? p.cap : p.scale) * kLog2e;
     slope = apart ? p.slopes[head] * kLog2e : 0.f;
-    scaled = !bent && (apart || !(p.scale > 0.f));      // products stand for scores in the order of their size
+    scaled = !bent;
   }
-  __device__ __forceinline__ bool as_they_are() const { return !bent && !scaled; }
+};
+// Nothing but a positive factor: the products stand for the scores, in the order of their size.  Kernels of their own, which have
+// registers for more waves.
+template <>
+struct Scores<true> {
+  float factor;
+  static constexpr float tanh_scale = 0.f, slope = 0.f;
+  static constexpr bool bent = false, apart = false, scaled = false;
+  __device__ __forceinline__ Scores(const AttnLaunch &p, int) : factor(p.scale * kLog2e) {}
 };
 // tanh(x) = 1 - 2 r with r = 1 / (exp(2 x) + 1), whose derivative is 4 (r - r^2): 16-bit types carry r - r^2 and the factor at the end.
 template <typename Tag> constexpr float kBendFactor = Tag::kBytes == 4 ? 1.f : 4.f;
@@ -265,8 +275,8 @@ __device__ __forceinline__ float distance(f32x2 a, f32x2 b) {
 // Scores of N blocks of 16 rows, from the products in s.  What a call has is the same for all lanes: a loop for each, not a question
 // for each score.  Forward; `point` and what point_of(n, r) gives, the rows' positions, come multiplied by the slope where `stretched`
 // says so.
-template <typename Tag, int N, int CF, typename Points>
-__device__ __forceinline__ void finish_scores(const Scores &scores, bool stretched, f32x4 (&s)[N][CF], const f32x2 (&point)[CF], Points point_of) {
+template <typename Tag, bool PLAIN, int N, int CF, typename Points>
+__device__ __forceinline__ void finish_scores(const Scores<PLAIN> &scores, bool stretched, f32x4 (&s)[N][CF], const f32x2 (&point)[CF], Points point_of) {
   if (scores.bent) {
     const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
 #pragma unroll
@@ -307,10 +317,10 @@ __device__ __forceinline__ void finish_scores(const Scores &scores, bool stretch
 }
 // Backward: weights of 32 rows without what is not seen, from the products in s and the rows' or columns' logarithms; the distances,
 // and the tanh's derivative over kBendFactor.  seen(): masks s in place, before the exponential.
-template <typename Tag, int CF, typename Points, typename Lse, typename Seen>
-__device__ __forceinline__ void form_weights(const Scores &scores, f32x4 (&s)[2][CF], f32x4 (&far)[2][CF], f32x4 (&bend)[2][CF], const f32x2 (&point)[CF],
+template <typename Tag, bool PLAIN, int CF, typename Points, typename Lse, typename Seen>
+__device__ __forceinline__ void form_weights(const Scores<PLAIN> &scores, f32x4 (&s)[2][CF], f32x4 (&far)[2][CF], f32x4 (&bend)[2][CF], const f32x2 (&point)[CF],
                                              Points point_of, Lse lse, Seen seen) {
-  if (scores.as_they_are()) {
+  if constexpr (PLAIN) {
     seen();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -558,9 +568,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
   const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
   const int first = at.chunk * split.chunk_rows, last = min(p.nk, first + split.chunk_rows);
   const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
-  const Scores scores(p, at.head);
-  const bool plain = scores.as_they_are(), masked = p.k_segments != nullptr;
-  const float factor = plain ? scores.factor : 1.f;
+  const Scores<S::kPlain> scores(p, at.head);
+  const bool masked = p.k_segments != nullptr;
+  const float factor = S::kPlain ? scores.factor : 1.f;
   // without a cap the product's factor and the distance are one operation, if the positions carry the slope
   const bool stretched = scores.apart && !scores.bent && scores.slope >= 0.f;
   const float stretch = stretched ? scores.slope : 1.f;
@@ -631,7 +641,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
       }
     }
     const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block0 * 16 + 4 * g;
-    finish_scores<Tag, S::kRowBlocks, S::CF>(scores, stretched, s, point, [&](int n, int r) { return points[n * 16 + r]; });
+    finish_scores<Tag, S::kPlain, S::kRowBlocks, S::CF>(scores, stretched, s, point, [&](int n, int r) { return points[n * 16 + r]; });
     if (!every)
 #pragma unroll
       for (int n = 0; n < S::kRowBlocks; ++n) {
@@ -875,7 +885,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
   const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
   const int first = at.chunk * parts.chunk_rows, last = min(p.nk, first + parts.chunk_rows);
   const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
-  const Scores scores(p, at.head);
+  const Scores<S::kPlain> scores(p, at.head);
   const bool masked = p.k_segments != nullptr;
 
   u32x4 q[S::CF][S::kSlices], go[S::CF][S::kSlices];
@@ -984,7 +994,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
       const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
       const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
       const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
-      form_weights<Tag, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int, int, int f) { return lse[f]; }, [&] {
+      form_weights<Tag, S::kPlain, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int, int, int f) { return lse[f]; }, [&] {
         if (every) return;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -1126,7 +1136,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
 
   for (int head = head0; head < head0 + heads_here; ++head) {
     const HeadRows queries = head_rows<Tag>(p.q, at.b, head), grads = head_rows<Tag>(p.grad_out, at.b, head);
-    const Scores scores(p, head);
+    const Scores<S::kPlain> scores(p, head);
     TileLoads<S> next_q, next_g;
     RowLoads next = {};
     auto request = [&](int row0) {
@@ -1185,7 +1195,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
         const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
         const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
         const float *lse = reinterpret_cast<const float *>(tile + S::kLse) + block * 16 + 4 * g;
-        form_weights<Tag, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int h, int r, int) { return lse[h * 16 + r]; },
+        form_weights<Tag, S::kPlain, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int h, int r, int) { return lse[h * 16 + r]; },
                                  [&] {
                                    if (every) return;
 #pragma unroll
@@ -1283,21 +1293,21 @@ Mode column_mode(long long heads, int columns, bool masked) {
 }
 // Rows of a tile and sixteens of columns a wave, by the bytes of a row: narrow rows make long tiles; a wave with two sixteens reads half as
 // much LDS, but backward it has no room for rows of 256 bytes (the gradients' kernels, 16 heads of 128, 4096 queries, 16 bits: 1560 us for 857).
-template <typename Tag, int W>
+template <typename Tag, bool PLAIN, int W>
 struct ForwardModes {
   static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 256 ? 1 : 2;
-  typedef Shape<Tag, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
-  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 256 ? 1 : 2), kTwo, 4> Columns64;
-  typedef Shape<Tag, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), (kBytes > 128 ? 1 : 2), 4> Columns32;
-  typedef Shape<Tag, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 256 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), (kBytes > 128 ? 1 : 2), 4> Columns32;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
 };
-template <typename Tag, int W>
+template <typename Tag, bool PLAIN, int W>
 struct BackwardModes {
   static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 128 ? 1 : 2;
-  typedef Shape<Tag, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
-  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
-  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), kTwo, 4> Columns32;
-  typedef Shape<Tag, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), kTwo, 4> Columns32;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
 };
 
 template <typename S, typename... A>
@@ -1428,9 +1438,9 @@ hipError_t grad_kv_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
   return hipGetLastError();
 }
 
-template <typename Tag, int W>
+template <typename Tag, bool PLAIN, int W>
 hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  typedef ForwardModes<Tag, W> M;
+  typedef ForwardModes<Tag, PLAIN, W> M;
   switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr)) {
     case kColumns128: return forward_shape<typename M::Columns128>(p, stream, bytes);
     case kColumns64: return forward_shape<typename M::Columns64>(p, stream, bytes);
@@ -1439,9 +1449,9 @@ hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
   }
 }
 
-template <typename Tag, int W>
+template <typename Tag, bool PLAIN, int W>
 hipError_t backward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  typedef BackwardModes<Tag, W> M;
+  typedef BackwardModes<Tag, PLAIN, W> M;
   const bool keys = bytes != nullptr || p.grad_k != nullptr || p.grad_v != nullptr;
   size_t q_bytes = 0, kv_bytes = 0;
   hipError_t e = hipSuccess;
@@ -1462,15 +1472,25 @@ hipError_t backward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes
   return e;
 }
 
+bool plain_scores(const AttnLaunch &p) { return p.cap == 0.f && p.slopes == nullptr && p.scale > 0.f; }
+
+template <typename Tag, bool PLAIN>
+hipError_t forward_scores(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  if (p.width <= 32) return forward_width<Tag, PLAIN, 32>(p, stream, bytes);
+  return p.width <= 64 ? forward_width<Tag, PLAIN, 64>(p, stream, bytes) : forward_width<Tag, PLAIN, 128>(p, stream, bytes);
+}
 template <typename Tag>
 hipError_t forward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  if (p.width <= 32) return forward_width<Tag, 32>(p, stream, bytes);
-  return p.width <= 64 ? forward_width<Tag, 64>(p, stream, bytes) : forward_width<Tag, 128>(p, stream, bytes);
+  return plain_scores(p) ? forward_scores<Tag, true>(p, stream, bytes) : forward_scores<Tag, false>(p, stream, bytes);
+}
+template <typename Tag, bool PLAIN>
+hipError_t backward_scores(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
+  if (p.width <= 32) return backward_width<Tag, PLAIN, 32>(p, stream, bytes);
+  return p.width <= 64 ? backward_width<Tag, PLAIN, 64>(p, stream, bytes) : backward_width<Tag, PLAIN, 128>(p, stream, bytes);
 }
 template <typename Tag>
 hipError_t backward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  if (p.width <= 32) return backward_width<Tag, 32>(p, stream, bytes);
-  return p.width <= 64 ? backward_width<Tag, 64>(p, stream, bytes) : backward_width<Tag, 128>(p, stream, bytes);
+  return plain_scores(p) ? backward_scores<Tag, true>(p, stream, bytes) : backward_scores<Tag, false>(p, stream, bytes);
 }
 
 }  // namespace
