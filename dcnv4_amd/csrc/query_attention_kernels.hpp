@@ -628,17 +628,24 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_ke
   };
   auto work = [&](const char *tile, bool every) {
     const int block0 = row_wave * S::kRowBlocks;
+    // a block's fragments are read while the one before is multiplied; said so, for the compiler reads each where it is used and waits
     f32x4 s[S::kRowBlocks][S::CF];
+    u32x4 a[2][S::kSlices];
+#pragma unroll
+    for (int sl = 0; sl < S::kSlices; ++sl) a[0][sl] = fragment<S>(tile, block0, sl, lane);
 #pragma unroll
     for (int n = 0; n < S::kRowBlocks; ++n) {
+      if (n + 1 < S::kRowBlocks) {
+#pragma unroll
+        for (int sl = 0; sl < S::kSlices; ++sl) a[(n + 1) & 1][sl] = fragment<S>(tile, block0 + n + 1, sl, lane);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int f = 0; f < S::CF; ++f) s[n][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int sl = 0; sl < S::kSlices; ++sl) {
-        const u32x4 a = fragment<S>(tile, block0 + n, sl, lane);
+      for (int sl = 0; sl < S::kSlices; ++sl)
 #pragma unroll
-        for (int f = 0; f < S::CF; ++f) s[n][f] = mfma_64_bytes<Tag>(a, q[f][sl], s[n][f]);
-      }
+        for (int f = 0; f < S::CF; ++f) s[n][f] = mfma_64_bytes<Tag>(a[n & 1][sl], q[f][sl], s[n][f]);
     }
     const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block0 * 16 + 4 * g;
     finish_scores<Tag, S::kPlain, S::kRowBlocks, S::CF>(scores, stretched, s, point, [&](int n, int r) { return points[n * 16 + r]; });
