@@ -178,38 +178,56 @@ struct Weights {
     return Weights(left);
   }
 };
-// acc[d][f] += rows 16 block .. + 31 of the tensor, turned, times the weights, and where SETS is 2 times more weights
-template <typename S, int SETS = 1>
-__device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF], const char *tensor, int block, const Weights<S> &w, const Weights<S> &more, int lane) {
-  typedef typename S::Tag Tag;
-  const int g = lane >> 4, c = lane & 15;
-  if constexpr (Tag::kBytes == 2) {
-#pragma unroll
-    for (int d = 0; d < S::kWidthBlocks; ++d) {
+// Rows 16 block .. + 31 of a tensor with rows and width exchanged, sixteens d of the width: a lane's first operand.
+template <typename S>
+struct Turned {
+  static constexpr bool kHalf = S::Tag::kBytes == 2;
+  u32x4 half;
+  float full[kHalf ? 1 : 2][4];
+  __device__ __forceinline__ void read(const char *tensor, int block, int d, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+    if constexpr (kHalf) {
       const char *at = tensor + d / 2 * S::RT * 64 + block * 1024 + (4 * g + (c >> 2)) * 64 + (((d & 1) * 2 + ((c & 3) >> 1)) ^ turned_by(g)) * 16 + (c & 1) * 8;
       typedef __attribute__((address_space(3))) s16x4 lds_words;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_words *)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_words *)(at + 1024));
       const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-      const u32x4 turned = {a.x, a.y, b.x, b.y};
+      half = u32x4{a.x, a.y, b.x, b.y};
+    } else {
 #pragma unroll
-      for (int f = 0; f < S::CF; ++f) {
-        acc[d][f] = mfma_64_bytes<Tag>(turned, w.half[f], acc[d][f]);
-        if constexpr (SETS == 2) acc[d][f] = mfma_64_bytes<Tag>(turned, more.half[f], acc[d][f]);
+      for (int h = 0; h < 2; ++h) {
+        const char *at = tensor + d * S::RT * 64 + (block + h) * 1024 + 4 * g * 64 + ((c >> 2) ^ turned_by(g)) * 16 + (c & 3) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) full[h][r] = *reinterpret_cast<const float *>(at + r * 64);
       }
     }
-  } else {
+  }
+};
+// acc[d][f] += those rows times the weights, and where SETS is 2 times more weights
+template <typename S, int SETS = 1>
+__device__ __forceinline__ void add_product(f32x4 (&acc)[S::kWidthBlocks][S::CF], const char *tensor, int block, const Weights<S> &w, const Weights<S> &more, int lane) {
+  typedef typename S::Tag Tag;
+  Turned<S> t[2];
+  t[0].read(tensor, block, 0, lane);
 #pragma unroll
-    for (int d = 0; d < S::kWidthBlocks; ++d)
+  for (int d = 0; d < S::kWidthBlocks; ++d) {
+    if (d + 1 < S::kWidthBlocks) {
+      t[(d + 1) & 1].read(tensor, block, d + 1, lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (Tag::kBytes == 2) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const char *at = tensor + d * S::RT * 64 + (block + half) * 1024 + 4 * g * 64 + ((c >> 2) ^ turned_by(g)) * 16 + (c & 3) * 4;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float a = *reinterpret_cast<const float *>(at + r * 64);
-#pragma unroll
-          for (int f = 0; f < S::CF; ++f) acc[d][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w.full[half][f][r], acc[d][f], 0, 0, 0);
-        }
+      for (int f = 0; f < S::CF; ++f) {
+        acc[d][f] = mfma_64_bytes<Tag>(t[d & 1].half, w.half[f], acc[d][f]);
+        if constexpr (SETS == 2) acc[d][f] = mfma_64_bytes<Tag>(t[d & 1].half, more.half[f], acc[d][f]);
       }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int f = 0; f < S::CF; ++f) acc[d][f] = __builtin_amdgcn_mfma_f32_16x16x4f32(t[d & 1].full[h][r], w.full[h][f][r], acc[d][f], 0, 0, 0);
+    }
   }
 }
 template <typename S>
