@@ -260,6 +260,41 @@ __device__ __forceinline__ float dot_16_bytes(u32x4 a, u32x4 b, float sum) {
   return sum;
 }
 
+// Products of 32 rows of two tensors of a tile with the columns' operands, on top of what is in s and t.  Fragments are read two slices
+// ahead of their products.
+template <typename S>
+__device__ __forceinline__ void two_products(const char *first, const char *second, int block, const u32x4 (&x)[S::CF][S::kSlices], const u32x4 (&y)[S::CF][S::kSlices],
+                                             f32x4 (&s)[2][S::CF], f32x4 (&t)[2][S::CF], int lane) {
+  typedef typename S::Tag Tag;
+  constexpr int kStep = S::kSlices > 1 ? 2 : 1, kSteps = 2 * S::kSlices / kStep;
+  u32x4 a[2][kStep], b[2][kStep];
+  auto read = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      const int at = k * kStep + i;
+      a[k & 1][i] = fragment<S>(first, block + at / S::kSlices, at % S::kSlices, lane);
+      b[k & 1][i] = fragment<S>(second, block + at / S::kSlices, at % S::kSlices, lane);
+    }
+  };
+  read(0);
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    if (k + 1 < kSteps) {
+      read(k + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      const int h = (k * kStep + i) / S::kSlices, sl = (k * kStep + i) % S::kSlices;
+#pragma unroll
+      for (int f = 0; f < S::CF; ++f) {
+        s[h][f] = mfma_64_bytes<Tag>(a[k & 1][i], x[f][sl], s[h][f]);
+        t[h][f] = mfma_64_bytes<Tag>(b[k & 1][i], y[f][sl], t[h][f]);
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- scores
 // Scores go into exp2, so they are in units of its exponent.  Without cap and distance that is one factor, which rides along where
 // the maximum is taken off.
@@ -1000,22 +1035,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
       const int block = row_wave * S::kRowBlocks + n;
       f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int f = 0; f < S::CF; ++f) {
           s[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
           t[h][f] = minus_delta[f];
         }
-#pragma unroll
-        for (int sl = 0; sl < S::kSlices; ++sl) {
-          const u32x4 a = fragment<S>(tile, block + h, sl, lane), b = fragment<S>(tile + S::kTensorBytes, block + h, sl, lane);
-#pragma unroll
-          for (int f = 0; f < S::CF; ++f) {
-            s[h][f] = mfma_64_bytes<Tag>(a, q[f][sl], s[h][f]);
-            t[h][f] = mfma_64_bytes<Tag>(b, go[f][sl], t[h][f]);
-          }
-        }
-      }
+      two_products<S>(tile, tile + S::kTensorBytes, block, q, go, s, t, lane);
       const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
       const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
       const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
@@ -1200,22 +1226,13 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_ke
         f32x4 s[2][S::CF], t[2][S::CF], far[2][S::CF], bend[2][S::CF];
         const f32x4 *minus_delta = reinterpret_cast<const f32x4 *>(tile + S::kDelta) + block * 4 + g;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int f = 0; f < S::CF; ++f) {
             s[h][f] = f32x4{0.f, 0.f, 0.f, 0.f};
             t[h][f] = minus_delta[h * 4];
           }
-#pragma unroll
-          for (int sl = 0; sl < S::kSlices; ++sl) {
-            const u32x4 a = fragment<S>(tile, block + h, sl, lane), b = fragment<S>(tile + S::kTensorBytes, block + h, sl, lane);
-#pragma unroll
-            for (int f = 0; f < S::CF; ++f) {
-              s[h][f] = mfma_64_bytes<Tag>(a, k[f][sl], s[h][f]);
-              t[h][f] = mfma_64_bytes<Tag>(b, v[f][sl], t[h][f]);
-            }
-          }
-        }
+        two_products<S>(tile, tile + S::kTensorBytes, block, k, v, s, t, lane);
         const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
         const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
         const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
