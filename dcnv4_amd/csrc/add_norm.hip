@@ -11,7 +11,7 @@
 //
 // Rows that all start on 16 bytes go in vectors of eight elements.  Others (an odd width, an odd offset) go element by element, neighbours
 // in neighbouring lanes: a 16-byte access that crosses its alignment costs twice (100000 x 1023, 16 bits, forward 283 us and backward 589
-// in unaligned vectors, 200 and 251 so; 1024 channels 148 and 228).  The backward reads four tensors for the one it writes, which
+// in unaligned vectors, 195 and 251 so; 1024 channels 147 and 222).  The backward reads four tensors for the one it writes, which
 // memory gives at some 4.5 TB/s, a copy 6.2; loads two rows ahead were slower (401408 x 112: 112 us for 98).
 //
 // The parameters' gradients are summed in registers down a workgroup's slab, over its teams through LDS, and over the workgroups by a
@@ -350,13 +350,19 @@ bool in_vectors(const AddNormLaunch &p) {
   return p.width % 8 == 0 && row_fits(p.x) && row_fits(p.residual) && fits(p.weight, 0) && fits(p.bias, 0) && fits(p.out, 0) && fits(p.sum, 0) &&
          fits(p.grad_out, 0) && fits(p.grad_sum, 0) && fits(p.grad_x, 0) && fits(p.grad_residual, 0);
 }
-// Elements a lane: sixteen of rows of more than 512, so that a wave holds a row of up to 1024 channels and meets no barrier.
-int lane_elements(const AddNormLaunch &p) { return p.width > 512 ? 16 : 8; }
+// Elements a lane: eight, and sixteen where a row needs more than 512 lanes of eight.  Sixteen also for many rows of 513 to 1024
+// channels: a wave then holds a row and meets no barrier, which pays once the waves are many (768 channels, 16 bits, 8 and 16: forward
+// of 5003 rows 10.4 and 10.3 us, of 40000 49.7 and 43.5; backward 14.6 and 17.8, 81 and 60).  The forward of rows that go element
+// by element stays at eight (20000 x 1001: 42 us and 68).
+int lane_elements(const AddNormLaunch &p, bool backward) {
+  if (p.width > 4096) return 16;
+  return p.width > 512 && p.width <= 1024 && p.rows > 16384 && (backward || in_vectors(p)) ? 16 : 8;
+}
 // Parameters in registers pay over several rows; workgroups enough to fill the chip come first.
-Geometry geometry(const AddNormLaunch &p, long long most_blocks) {
+Geometry geometry(const AddNormLaunch &p, int elements, long long most_blocks) {
   Geometry g;
   g.team = 1;
-  while (g.team * lane_elements(p) < p.width) g.team *= 2;
+  while (g.team * elements < p.width) g.team *= 2;
   g.threads = std::max(g.team, 64);
   if (g.team <= kWave && p.rows * g.team >= 256ll * 1024) g.threads = 256;
   const long long teams = g.threads / g.team, passes = (p.rows + teams - 1) / teams;
@@ -365,10 +371,10 @@ Geometry geometry(const AddNormLaunch &p, long long most_blocks) {
   g.blocks = (unsigned)((p.rows + g.slab - 1) / g.slab);
   return g;
 }
-Geometry forward_geometry(const AddNormLaunch &p) { return geometry(p, 4096); }
+Geometry forward_geometry(const AddNormLaunch &p) { return geometry(p, lane_elements(p, false), 4096); }
 Geometry backward_geometry(const AddNormLaunch &p) {
   // partial sums stay below 32 MB
-  return geometry(p, std::max<long long>(1, std::min<long long>(1024, (32ll << 20) / (8ll * p.width))));
+  return geometry(p, lane_elements(p, true), std::max<long long>(1, std::min<long long>(1024, (32ll << 20) / (8ll * p.width))));
 }
 
 template <typename T>
@@ -388,8 +394,9 @@ hipError_t run(const AddNormLaunch &p, hipStream_t stream, bool backward) {
 }
 template <typename X, typename R, bool WIDE>
 hipError_t with_types(const AddNormLaunch &p, hipStream_t stream, bool backward) {
-  if (in_vectors(p)) return lane_elements(p) == 8 ? run<Types<X, R, WIDE, 8, 1>>(p, stream, backward) : run<Types<X, R, WIDE, 8, 2>>(p, stream, backward);
-  return lane_elements(p) == 8 ? run<Types<X, R, WIDE, 1, 8>>(p, stream, backward) : run<Types<X, R, WIDE, 1, 16>>(p, stream, backward);
+  const int elements = lane_elements(p, backward);
+  if (in_vectors(p)) return elements == 8 ? run<Types<X, R, WIDE, 8, 1>>(p, stream, backward) : run<Types<X, R, WIDE, 8, 2>>(p, stream, backward);
+  return elements == 8 ? run<Types<X, R, WIDE, 1, 8>>(p, stream, backward) : run<Types<X, R, WIDE, 1, 16>>(p, stream, backward);
 }
 template <typename X>
 hipError_t with_residual(const AddNormLaunch &p, hipStream_t stream, bool backward) {

@@ -117,6 +117,12 @@ def test_rows(rows, width, dtype):
     check(make((rows, width), dtype, dtype, dtype, seed=rows))
 
 
+@pytest.mark.parametrize("dtype", (F32, F16), ids=IDS.get)
+@pytest.mark.parametrize("rows,width", [(16384, 513), (16385, 515), (16385, 520), (16390, 1024), (16390, 1032)])
+def test_many_rows_of_some_hundred_channels(rows, width, dtype):
+    check(make((rows, width), dtype, dtype, dtype, seed=rows))
+
+
 @pytest.mark.parametrize("stream", (False, True), ids=("post", "stream"))
 @pytest.mark.parametrize("width", (96, 333))
 @pytest.mark.parametrize("x,residual,params", [(F16, F32, F32), (F32, F16, F32), (BF16, F32, F32), (F32, BF16, BF16), (F16, F16, F32), (BF16, BF16, F32),
