@@ -76,8 +76,8 @@ Tensor attn_rows(const Tensor &t, const AttnShape &s) {
   if (s.padded() != s.width) return at::constant_pad_nd(t, {0, s.padded() - s.width}).contiguous();
   const int64_t size = t.element_size();
   bool fits = (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && (t.stride(3) == 1 || t.size(3) == 1);
-  // (64 rows of a tile are addressed in 31 bits)
-  for (int d = 0; d < 3; ++d) fits = fits && (t.size(d) <= 1 || (t.stride(d) * size % 16 == 0 && t.stride(d) * size < (1 << 24)));
+  // (the kernels address the up to 256 rows of a tile in 31 bits)
+  for (int d = 0; d < 3; ++d) fits = fits && (t.size(d) <= 1 || (t.stride(d) * size % 16 == 0 && (d != 1 || t.stride(d) * size < (1 << 23))));
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 AttnRows row_view(const Tensor &t) {

@@ -201,6 +201,25 @@ def test_a_memory_whose_offsets_pass_32_bits():
         assert torch.count_nonzero(a) == torch.count_nonzero(a[:, seen])
 
 
+@pytest.mark.parametrize("pitch", (5 << 10, (1 << 23) - 16, (1 << 23) + 16, 3 << 22))
+def test_tokens_that_lie_megabytes_apart(pitch):
+    # a tile of 128 or 256 rows reaches over 2 GB from its first one
+    n, l, m, d = 2, 600, 8, 32
+    t = on_gpu(inputs(n, l, l, m, m, d, F16, seed=24))
+    plain_leaves = leaves(t)
+    plain = call(t)
+    plain_grads = torch.autograd.grad(plain, plain_leaves, t["grad"])
+    memory = torch.empty(n * l * pitch // 2, dtype=F16, device="cuda")
+    far = dict(t)
+    for i, name in enumerate(("q", "k", "v", "grad")):
+        far[name] = memory.as_strided((n, l, m, d), (l * pitch // 2, pitch // 2, d, 1), i * m * d).copy_(t[name].detach())
+    far_leaves = [far[name].requires_grad_() for name in ("q", "k", "v")]
+    out = call(far)
+    assert torch.equal(out, plain)
+    for got, want in zip(torch.autograd.grad(out, far_leaves, far["grad"]), plain_grads):
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", (F16, BF16), ids=IDS.get)
 def test_gradients_of_tiny_and_of_large_size(dtype):
     for factor in (1e-4, 300.0):
