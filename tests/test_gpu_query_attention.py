@@ -112,6 +112,13 @@ def test_heads_that_share_a_key_head(m, mk, dtype):
     check(inputs(2, 50, 77, m, mk, 32, dtype, mask="padding", seed=m))
 
 
+@pytest.mark.parametrize("mask", ("none", "random"))
+@pytest.mark.parametrize("m,lk", [(8, 17000), (6, 9000)])
+def test_heads_that_share_a_key_head_of_a_long_memory(m, lk, mask):
+    # the heads in two parts of four, and in six of one
+    check(inputs(4, 40, lk, m, 1, 32, F16, mask=mask, seed=m), device="cuda")
+
+
 @pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
 @pytest.mark.parametrize("cap,distance", [(0.0, True), (3.0, False), (50.0, False), (8.0, True)])
 @pytest.mark.parametrize("mask", ("none", "random", "documents", "prefix", "nothing"))
