@@ -1351,7 +1351,7 @@ template <typename Tag, bool PLAIN, int W>
 struct BackwardModes {
   static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 128 ? 1 : 2;
   typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
   typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), kTwo, 4> Columns32;
   typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
 };
