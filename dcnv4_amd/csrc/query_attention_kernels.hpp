@@ -1326,14 +1326,15 @@ int row_lanes(const AttnLaunch &p) {
 // bits: 8 heads x 300 queries 12.1 / 13.1 / 9.8 / 7.6; 16 x 1100 20.9 / 19.2 / 25.8 / 29.7; 32 x 1100 28.7 / 31.0 / 38.8 / 49.5; 32 x 2500
 // 82 / 85 / 113 / 165.  The gradients' kernels go the same way: dK and dV 16.8 / 11.4 / 9.9 / 7.9 and 33.9 / 28.6 / 34.7 / 42.0 for the first two.
 enum Mode { kColumns128, kColumns64, kColumns32, kColumns16 };
-Mode column_mode(long long heads, int columns, bool masked, bool plain) {
+Mode column_mode(long long heads, int columns, bool masked, bool even) {
   // sequences that end within a tile cost the whole of it, and make workgroups of unequal work: 16 heads of 128, 5003 queries in sequences of
   // some hundred, forward with 128 columns 216 us, with 64 164
-  // scores with a cap or distances keep the vector units busy, and then two workgroups a CU should come out even: forward and dQ of 8 heads
-  // of 32 with distances, 2500 queries, 320 workgroups of 128 columns 95 and 103 us, 640 of 64 92 and 98; 7744 queries 488 for 276 and
-  // 299, 968 for 320 and 313; with a cap as well, 32 heads, 900 queries 256 for 38 and 40, 480 for 32 and 34
+  // two workgroups a CU should come out even, but for plain scores of heads above 64 channels, whose tiles cost more to bring in: forward and
+  // dQ of 8 heads, bf16, with distances, 32 channels, 2 x 2500 queries: 320 workgroups of 128 columns 95 and 103 us, 640 of 64 92 and 98;
+  // 7744 queries 488 for 276 and 299, 968 for 320 and 313; plain, 5000 queries 320 for 124 and 101, 632 for 112 and 81; of 128 channels 227
+  // for 232
   const long long blocks = heads * ceil_div(columns, 128), places = (blocks + 511) / 512 * 512;
-  if (blocks >= (masked ? 1024 : 256) && (plain || 4 * blocks >= 3 * places)) return kColumns128;
+  if (blocks >= (masked ? 1024 : 256) && (!even || 4 * blocks >= 3 * places)) return kColumns128;
   if (heads * ceil_div(columns, 64) >= 256) return kColumns64;
   return heads * ceil_div(columns, 32) >= 256 ? kColumns32 : kColumns16;
 }
@@ -1494,7 +1495,7 @@ hipError_t grad_kv_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
 template <typename Tag, bool PLAIN, int W>
 hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
   typedef ForwardModes<Tag, PLAIN, W> M;
-  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, PLAIN)) {
+  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, !PLAIN || W <= 64)) {
     case kColumns128: return forward_shape<typename M::Columns128>(p, stream, bytes);
     case kColumns64: return forward_shape<typename M::Columns64>(p, stream, bytes);
     case kColumns32: return forward_shape<typename M::Columns32>(p, stream, bytes);
@@ -1508,14 +1509,14 @@ hipError_t backward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes
   const bool keys = bytes != nullptr || p.grad_k != nullptr || p.grad_v != nullptr;
   size_t q_bytes = 0, kv_bytes = 0;
   hipError_t e = hipSuccess;
-  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, PLAIN)) {
+  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, !PLAIN || W <= 64)) {
     case kColumns128: e = grad_q_shape<typename M::Columns128>(p, stream, bytes ? &q_bytes : nullptr); break;
     case kColumns64: e = grad_q_shape<typename M::Columns64>(p, stream, bytes ? &q_bytes : nullptr); break;
     case kColumns32: e = grad_q_shape<typename M::Columns32>(p, stream, bytes ? &q_bytes : nullptr); break;
     default: e = grad_q_shape<typename M::Columns16>(p, stream, bytes ? &q_bytes : nullptr);
   }
   if (e != hipSuccess || !keys) return e;
-  switch (column_mode((long long)p.batch * p.kv_heads, p.nk, p.k_segments != nullptr, PLAIN)) {
+  switch (column_mode((long long)p.batch * p.kv_heads, p.nk, p.k_segments != nullptr, !PLAIN || W <= 64)) {
     case kColumns128: e = grad_kv_shape<typename M::Columns128>(p, stream, bytes ? &kv_bytes : nullptr); break;
     case kColumns64: e = grad_kv_shape<typename M::Columns64>(p, stream, bytes ? &kv_bytes : nullptr); break;
     case kColumns32: e = grad_kv_shape<typename M::Columns32>(p, stream, bytes ? &kv_bytes : nullptr); break;

@@ -159,6 +159,13 @@ def test_every_shape_of_workgroup(width, n, m, lq, mask, dtype):
     check(inputs(n, lq, lq, m, m, width, dtype, mask=mask, seed=width + m), device="cuda")
 
 
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("distance", (False, True))
+@pytest.mark.parametrize("width", (32, 64, 128))
+def test_workgroups_of_128_columns(width, distance, dtype):
+    check(inputs(3, 1030, 1030, 16, 16, width, dtype, distance=distance, seed=width), device="cuda")
+
+
 @pytest.mark.parametrize("width", (32, 64))
 def test_many_heads_with_masks(width):
     check(inputs(8, 1030, 1030, 16, 16, width, F16, mask="prefix", seed=width), device="cuda")
