@@ -57,7 +57,8 @@ def _fusable(x, residual, norm):
 def add_layer_norm(x, residual, norm, return_sum=False):
     """``norm(x + residual)`` for an ``nn.LayerNorm`` over the last axis; ``residual`` of x's shape, or None.  The result has the
     wider type of the two, float32 under autocast as torch's own layer norm there.  With ``return_sum`` also the sum, in the wider type:
-    ``(result, x + residual)``, the stream of a pre-norm network."""
+    ``(result, x + residual)``, the stream of a pre-norm network.  The backward reads x and residual again: neither is to be changed in
+    place before it."""
     weight, bias, wide = norm.weight, norm.bias, torch.is_autocast_enabled()
     if weight is not None or tuple(norm.normalized_shape) == (x.shape[-1],):      # (the weight says as much)
         output = _native.add_layer_norm(x, residual, weight, bias, norm.eps, wide, return_sum)
