@@ -71,6 +71,10 @@ struct Shape {
   // two waves a SIMD at least, which also keeps the matrix instructions' results out of the accumulation registers and their copies;
   // the largest tiles leave room for one
   static constexpr int kWavesPerSimd = W * Tag::kBytes > 256 ? 1 : 2;
+  // narrow heads by 64 columns: three where that costs next to no scratch memory.  32 channels, bf16: forward of 32 heads, 2500 queries 92 -> 83
+  // us, with distances 122 -> 112; dK and dV of bf16 96 -> 87 (fp16, with its scales a column, or distances: spills, 32 -> 40)
+  static constexpr bool kNarrow = W * Tag::kBytes <= 64 && RW == 2;
+  static constexpr int kForwardWaves = kNarrow ? 3 : kWavesPerSimd, kGradKvWaves = kNarrow && kPlain && Tag::kCode == BF16::kCode ? 3 : kWavesPerSimd;
   static constexpr int kLdsBytes = std::max(2 * kTileBytes, kMergeBytes);
   static_assert(kRowBlocks % 2 == 0 && kCarried * kWaves * 16 == RT && kLdsBytes <= 156 * 1024);
 };
@@ -610,7 +614,7 @@ struct Split {
 
 // TRAIN: a backward follows (16-bit types; fp32 ones have nothing to round).
 template <typename S, bool TRAIN>
-__global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_forward_kernel(const AttnLaunch p, const Split split) {
+__global__ void __launch_bounds__(S::kThreads, S::kForwardWaves) attn_forward_kernel(const AttnLaunch p, const Split split) {
   typedef typename S::Tag Tag;
   extern __shared__ __align__(16) char lds[];
   __shared__ char s_flags[64];
@@ -1146,7 +1150,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
 
 // dK and dV: columns are keys, rows the queries of every head that shares the key head.
 template <typename S>
-__global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_kv_kernel(const AttnLaunch p, const BackwardParts parts) {
+__global__ void __launch_bounds__(S::kThreads, S::kGradKvWaves) attn_grad_kv_kernel(const AttnLaunch p, const BackwardParts parts) {
   typedef typename S::Tag Tag;
   extern __shared__ __align__(16) char lds[];
   __shared__ char s_flags[64];
