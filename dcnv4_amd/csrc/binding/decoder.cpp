@@ -54,6 +54,9 @@ AttnShape attn_check(const AttnInputs &a) {
   // rows are counted in 32 bits by the kernels
   if (s.nq > (1 << 30) || s.nk > (1 << 30)) raise_runtime("sequences of more than 2^30 tokens");
   if (s.batch * s.nq * s.heads > kIntMax || s.batch * s.nk * s.kv_heads > kIntMax) raise_runtime("more than 2^31 - 1 rows of queries or keys");
+  // a launch has fewer than 2^32 threads: workgroups of 256 for 128 tokens of a head
+  if (s.batch * s.heads * ((s.nq + 127) / 128) >= 1 << 24 || s.batch * s.kv_heads * ((s.nk + 127) / 128) >= 1 << 24)
+    raise_runtime("more than 2^24 - 1 pieces of 128 queries or keys of a head");
   if (!(std::fabs(a.scale) < kFloatMax)) raise_runtime("scale must be finite");
   if (a.cap != 0.f && !(a.cap >= 1e-30f && a.cap <= 1e30f)) raise_runtime("cap must be zero (none) or between 1e-30 and 1e30");
   if (a.q_segments.defined()) {

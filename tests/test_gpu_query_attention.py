@@ -502,3 +502,12 @@ def test_refusals():
     refused("scale", scale=float("nan"))
     refused("cap", cap=float("inf"))
     refused("cap", cap=float("nan"))
+
+
+def test_batches_beyond_a_launch_are_refused():
+    from dcnv4_amd.functions import query_attention
+    one = torch.zeros(1, 1, 1, 8, dtype=F16, device="cuda")
+    for shape, match in (((1 << 21, 1, 8, 8), "24 - 1 pieces"), ((1 << 20, 129, 8, 8), "24 - 1 pieces"), ((1 << 20, 300, 8, 8), "31 - 1 rows")):
+        many = one.expand(shape)      # refused before anything is allocated
+        with pytest.raises(RuntimeError, match=match):
+            query_attention(many, many, many)
