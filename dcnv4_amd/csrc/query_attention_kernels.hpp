@@ -300,13 +300,27 @@ __device__ __forceinline__ void two_products(const char *first, const char *seco
 }
 
 // ---------------------------------------------------------------- scores
+// 16-bit types form cap tanh(x / cap) as cap - 2 cap / (exp(2 x / cap) + 1), four instructions whose error is that of numbers of the cap's size:
+// at most 2^-20 cap (a last bit of exponential and reciprocal each, the sum's half), which the weights show.  At 256 that is half a rounding
+// of fp16's weights; higher caps take a form that is exact for small x / cap.
+constexpr float kQuickCap = 256.f;
+// To a relative 2^-21: a series whose next term is 3e-7 at 1/4, and beyond it (1 - e) / (1 + e) with e = exp(-2 |x|), which loses no digits there.
+// fp32 results see the last bits, which tanhf has.  16-bit types do without its registers: kernels that keep some in scratch memory already
+// would keep a dozen more.
+template <typename Tag>
+__device__ __forceinline__ float exact_tanh(float x) {
+  if constexpr (Tag::kBytes == 4) return tanhf(x);
+  const float e = __builtin_amdgcn_exp2f(fabsf(x) * (-2.f * kLog2e)), z = x * x;
+  const float near = fmaf(fmaf(fmaf(z, -17.f / 315.f, 2.f / 15.f), z, -1.f / 3.f), z * x, x);
+  return fabsf(x) < 0.25f ? near : copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
+}
 // Scores go into exp2, so they are in units of its exponent.  Without cap and distance that is one factor, which rides along where
 // the maximum is taken off.
 template <bool PLAIN>
 struct Scores {
   float tanh_scale, factor, slope;
-  bool bent, apart, scaled;      // there is a cap; a distance; neither, but a factor that cannot ride along
-  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : bent(p.cap > 0.f), apart(p.slopes != nullptr) {
+  bool bent, high, apart, scaled;      // there is a cap; one above kQuickCap; a distance; neither, but a factor that cannot ride along
+  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : bent(p.cap > 0.f), high(p.cap > kQuickCap), apart(p.slopes != nullptr) {
     tanh_scale = bent ? p.scale / p.cap : 0.f;
     factor = (bent ? p.cap : p.scale) * kLog2e;
     slope = apart ? p.slopes[head] * kLog2e : 0.f;
@@ -319,7 +333,7 @@ template <>
 struct Scores<true> {
   float factor;
   static constexpr float tanh_scale = 0.f, slope = 0.f;
-  static constexpr bool bent = false, apart = false, scaled = false;
+  static constexpr bool bent = false, high = false, apart = false, scaled = false;
   __device__ __forceinline__ Scores(const AttnLaunch &p, int) : factor(p.scale * kLog2e) {}
 };
 // tanh(x) = 1 - 2 r with r = 1 / (exp(2 x) + 1), whose derivative is 4 (r - r^2): 16-bit types carry r - r^2 and the factor at the end.
@@ -336,15 +350,21 @@ template <typename Tag, bool PLAIN, int N, int CF, typename Points>
 __device__ __forceinline__ void finish_scores(const Scores<PLAIN> &scores, bool stretched, f32x4 (&s)[N][CF], const f32x2 (&point)[CF], Points point_of) {
   if (scores.bent) {
     const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
+    if (Tag::kBytes == 4 || scores.high) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int f = 0; f < CF; ++f)
+        for (int f = 0; f < CF; ++f)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (Tag::kBytes == 4) s[n][f][r] = tanhf(s[n][f][r] * scores.tanh_scale) * scores.factor;      // fp32 results see the last bits
-          else s[n][f][r] = fmaf(twice, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][f][r] * rate) + 1.f), scores.factor);
-        }
+          for (int r = 0; r < 4; ++r) s[n][f][r] = exact_tanh<Tag>(s[n][f][r] * scores.tanh_scale) * scores.factor;
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int f = 0; f < CF; ++f)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[n][f][r] = fmaf(twice, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[n][f][r] * rate) + 1.f), scores.factor);
+    }
   }
   if (stretched) {
 #pragma unroll
@@ -389,22 +409,30 @@ __device__ __forceinline__ void form_weights(const Scores<PLAIN> &scores, f32x4 
   }
   if (scores.bent) {
     const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
+    if (Tag::kBytes == 4 || scores.high) {
+      constexpr float bend0 = 1.f / kBendFactor<Tag>;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int f = 0; f < CF; ++f)
+        for (int f = 0; f < CF; ++f)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if constexpr (Tag::kBytes == 4) {
-            const float t = tanhf(s[h][f][r] * scores.tanh_scale);
-            bend[h][f][r] = fmaf(-t, t, 1.f);
+          for (int r = 0; r < 4; ++r) {
+            const float t = exact_tanh<Tag>(s[h][f][r] * scores.tanh_scale);
+            bend[h][f][r] = fmaf(t * -bend0, t, bend0);
             s[h][f][r] = fmaf(t, scores.factor, -lse(h, r, f));
-          } else {
+          }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int f = 0; f < CF; ++f)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
             const float t = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[h][f][r] * rate) + 1.f);
             bend[h][f][r] = fmaf(-t, t, t);
             s[h][f][r] = fmaf(twice, t, scores.factor - lse(h, r, f));
           }
-        }
+    }
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h)

@@ -23,9 +23,12 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
 
     What a kernel rounds to the type: each weight of P before its product (unit P, and tiny against the largest of a row), each
     dS before its product, delta through the rounded out, and the result.  All else is fp32: a score from `width` products is off by
-    e = (width + 8) 2^-24 times the sum of their sizes (cap, slope times distance and the score itself counted in), a weight by 2 e and
-    the sum over the keys, relatively.  The scale of dS in fp16 keeps it below 2^15 by width max|g| max|v|, so that tiny weighs 2^-15 of
-    twice that.  Sizes are floats of all heads, key heads already spread over the heads that share them."""
+    e = (width + 8) 2^-24 times the sum of their sizes (slope times distance and the score itself counted in), a weight by 2 e and
+    the sum over the keys, relatively.  A tanh is off relative to itself, no more than the product that goes into it; where results have 16 bits and
+    the cap is at most 256 a kernel may form it as the difference of numbers of the cap's size, e then has 2^-20 of the cap as well.
+    Exponentials have no subnormals: a weight below 2^-126 may be zero, in the forward against a maximum that is up to 2^8 behind, so 2^-118 of
+    the largest, in the backward against the row's sum; dS below that too.  The scale of dS in fp16 keeps it below 2^15 by
+    width max|g| max|v|, so that tiny weighs 2^-15 of twice that.  Sizes are floats of all heads, key heads already spread over the heads that share them."""
     to = lambda t: t.detach().to(device).double()
     q, k, v = to(q), to(k), to(v)
     n, lq, m, d = q.shape
@@ -40,7 +43,6 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
     if cap:
         th = torch.tanh(x / cap)
         s = cap * th
-        size = size + cap
     dist = torch.zeros(n, 1, lq, lk, dtype=torch.float64, device=device)
     if slopes is not None:
         pq, pk = to(q_points), to(k_points)
@@ -63,11 +65,12 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
         return torch.where(torch.isfinite(t), t, 0.0)
 
     kh, vh, qh = clean(kh), clean(vh), clean(qh)
-    error = torch.where(see, 2.0 ** -24 * (2 * (d + 8) * clean(size) + lk + 64), 0.0).amax(-1, keepdim=True) if lk else torch.zeros_like(top)
+    bent_off = 2.0 ** -20 * cap if unit > 2.0 ** -20 and cap <= 256 else 0.0
+    error = torch.where(see, 2.0 ** -24 * (2 * (d + 8) * clean(size) + lk + 64) + 2 * bent_off, 0.0).amax(-1, keepdim=True) if lk else torch.zeros_like(top)
     out = p @ vh
     back = lambda t: t.permute(0, 2, 1, 3)
     gather = lambda t: back(t.reshape(n, k.shape[2], share, lk, -1).sum(2))
-    found = {"out": (back(out), back(unit * out.abs() + (2 * unit + error) * (p @ vh.abs()) + tiny * (see.double() @ vh.abs())) + tiny)}
+    found = {"out": (back(out), back(unit * out.abs() + (2 * unit + error) * (p @ vh.abs()) + (tiny + 2.0 ** -118) * (see.double() @ vh.abs())) + tiny)}
     if grad is None:
         return found
     g = clean(to(grad).permute(0, 2, 1, 3))
@@ -80,13 +83,13 @@ def attention(q, k, v, grad=None, scale=None, cap=0.0, q_segments=None, k_segmen
     most = g.abs().max() * vh.abs().max() * d if g.numel() and vh.numel() else 0.0
     # of dS, dX and what they are multiplied by
     off = p * (unit * about + 2 * error * (g.abs() @ vh.abs().transpose(-1, -2) + about))
-    off = off + (unit * ds.abs() + see.double() * tiny * 2.0 ** -15 * most)
+    off = off + (unit * ds.abs() + see.double() * (tiny * 2.0 ** -15 * most + 2.0 ** -126 * (1 + g.abs() @ vh.abs().transpose(-1, -2) + about)))
     bend = ds.abs() * torch.where(see, error, 0.0) * (2.0 if cap else 0.0)
     dq, dk, dv = scale * (dx @ kh), scale * (dx.transpose(-1, -2) @ qh), p.transpose(-1, -2) @ g
     spot = unit * dx.abs() + off + bend
     found["grad_query"] = (back(dq), back(unit * dq.abs() + abs(scale) * (spot @ kh.abs())) + tiny)
     found["grad_key"] = (gather(dk), gather(2 * unit * dk.abs() + abs(scale) * (spot.transpose(-1, -2) @ qh.abs())) + tiny)
-    weight_off = p * (unit + 2 * error) + see.double() * tiny * 2.0 ** -8
+    weight_off = p * (unit + 2 * error) + see.double() * (tiny * 2.0 ** -8 + 2.0 ** -126)
     found["grad_value"] = (gather(dv), gather(2 * unit * dv.abs() + weight_off.transpose(-1, -2) @ g.abs()) + tiny)
     if slopes is not None:
         dist = clean(dist)
