@@ -1,8 +1,9 @@
-"""query_attention's scores at the ends of their range: caps from a few units to the largest that is taken."""
+"""query_attention's scores at the ends of their range: caps from a few units to the largest that is taken, positions far from zero, slopes of
+any size."""
 import pytest
 import torch
 
-from tests.test_gpu_query_attention import BF16, F16, F32, IDS, check, inputs
+from tests.test_gpu_query_attention import BF16, F16, F32, IDS, call, check, inputs, leaves, on_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +23,47 @@ def test_scores_that_a_large_cap_bends(cap, dtype):
     t = inputs(1, 150, 150, 2, 2, 16, dtype, seed=42)
     check(t, scale=20.0, cap=cap)
     check(t, scale=-1.0, cap=cap)
+
+
+def placed(t, gen, offset, step=1 / 16, extent=800):
+    """Points on a grid that fp32 holds exactly, so that two of them are as far apart wherever the grid begins."""
+    n, lq, lk = t["q"].shape[0], t["q"].shape[1], t["k"].shape[1]
+    offset = torch.tensor(offset, dtype=F32)
+    for name, length in (("q_points", lq), ("k_points", lk)):
+        t[name] = torch.randint(0, extent, (n, length, 2), generator=gen) * step + offset
+    return t
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("cap", (0.0, 30.0))
+@pytest.mark.parametrize("slope", (0.3, 1.0, 16.0, 1e-7, -0.7))
+def test_distances_do_not_depend_on_where_the_points_lie(slope, cap, dtype):
+    found = []
+    for offset in ((0, 0), (1300, 700), (-20000, 100)):
+        t = on_gpu(placed(inputs(2, 130, 150, 2, 2, 32, dtype, distance=True, seed=43), torch.Generator().manual_seed(5), offset))
+        t["slopes"] = torch.full((2,), slope, device="cuda")
+        wanted = leaves(t)
+        out = call(t, cap=cap)
+        found.append((out, *torch.autograd.grad(out, wanted, t["grad"])))
+    for other in found[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(found[0], other))
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("mask", ("none", "random"))
+def test_distances_in_pixels(mask, dtype):
+    t = inputs(2, 130, 150, 6, 3, 32, dtype, mask=mask, distance=True, seed=44)
+    placed(t, torch.Generator().manual_seed(6), (1000, 1000))
+    t["slopes"] = torch.tensor([1e-3, 0.05, 1.0, 1.3, 16.0, 300.0])
+    check(t)
+
+
+# Slopes about where scores change their units: 2^20 times the product's factor and 2^-20 of it; and far beyond.
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("scale", (0.17, -0.17, 0.0))
+def test_slopes_of_any_size(scale, dtype):
+    t = inputs(1, 90, 110, 12, 12, 32, dtype, distance=True, seed=45)
+    t["slopes"] = torch.tensor([0.0, 1e-40, 1e-30, 1.5e-7, 1.7e-7, 2e-7, 1.7e5, 1.8e5, 2e5, 1e10, 1e25, -1e-30])
+    t["k_points"][:, :45] = t["q_points"][:, 45:]          # some of the points meet
+    t["q_points"][:, :45] = t["k_points"][:, :45]
+    check(t, scale=scale)
