@@ -1,6 +1,7 @@
 // What stands between the sampling layers of a deformable decoder: attention among queries and the normalised sum.  Checks, dense
 // rows where the kernels need them, allocation and autograd nodes.
 #include <cmath>
+#include <tuple>
 
 #include "../add_norm.hpp"
 #include "../query_attention.hpp"
@@ -54,9 +55,15 @@ AttnShape attn_check(const AttnInputs &a) {
   // rows are counted in 32 bits by the kernels
   if (s.nq > (1 << 30) || s.nk > (1 << 30)) raise_runtime("sequences of more than 2^30 tokens");
   if (s.batch * s.nq * s.heads > kIntMax || s.batch * s.nk * s.kv_heads > kIntMax) raise_runtime("more than 2^31 - 1 rows of queries or keys");
-  // a launch has fewer than 2^32 threads: workgroups of 256 for 128 tokens of a head
-  if (s.batch * s.heads * ((s.nq + 127) / 128) >= 1 << 24 || s.batch * s.kv_heads * ((s.nk + 127) / 128) >= 1 << 24)
-    raise_runtime("more than 2^24 - 1 pieces of 128 queries or keys of a head");
+  // the kernels address the rows of a tile, up to 256, in 31 bits; dense tensors, among them the result, have all heads between rows
+  const int64_t row_bytes = s.padded() * a.q.element_size();
+  for (const auto &[tokens, heads, name] : {std::tuple{s.nq, s.heads, "query"}, std::tuple{s.nk, s.kv_heads, "key"}})
+    if (tokens > 1 && std::min<int64_t>(tokens, 256) * heads * row_bytes > kIntMax)
+      raise_runtime("%lld heads of the %s: %lld tokens in a row reach over more than 2^31 - 1 bytes", (long long)heads, name, (long long)std::min<int64_t>(tokens, 256));
+  // a launch has fewer than 2^32 threads: workgroups of 256 for 128 tokens of a head, of the wider rows 64
+  const int64_t piece = row_bytes > 128 ? 64 : 128;
+  if (s.batch * s.heads * ((s.nq + piece - 1) / piece) >= 1 << 24 || s.batch * s.kv_heads * ((s.nk + piece - 1) / piece) >= 1 << 24)
+    raise_runtime("more than 2^24 - 1 pieces of %lld queries or keys of a head", (long long)piece);
   if (!(std::fabs(a.scale) < kFloatMax)) raise_runtime("scale must be finite");
   if (a.cap != 0.f && !(a.cap >= 1e-30f && a.cap <= 1e30f)) raise_runtime("cap must be zero (none) or between 1e-30 and 1e30");
   if (a.q_segments.defined()) {
@@ -79,7 +86,7 @@ Tensor attn_rows(const Tensor &t, const AttnShape &s) {
   if (s.padded() != s.width) return at::constant_pad_nd(t, {0, s.padded() - s.width}).contiguous();
   const int64_t size = t.element_size();
   bool fits = (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && (t.stride(3) == 1 || t.size(3) == 1);
-  // (the kernels address the up to 256 rows of a tile in 31 bits)
+  // (the kernels address the up to 256 rows of a tile in 31 bits; a copy's do as far as attn_check lets pass)
   for (int d = 0; d < 3; ++d) fits = fits && (t.size(d) <= 1 || (t.stride(d) * size % 16 == 0 && (d != 1 || t.stride(d) * size < (1 << 23))));
   return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }

@@ -1,0 +1,53 @@
+"""What query_attention and add_layer_norm make of calls at the ends of what they take, and of what a program has put around them."""
+import pytest
+import torch
+
+from oracle import query_attention as oracle_attention
+from tests.test_gpu_query_attention import BF16, F16, F32, IDS, TINY, UNIT, close
+
+pytestmark = pytest.mark.gpu
+
+
+def test_heads_whose_rows_lie_too_far_apart_are_refused():
+    from dcnv4_amd.functions import query_attention
+
+    def refused(match, lq, lk, m, mk, d, dtype=F16, n=1):
+        one = torch.zeros(1, 1, 1, d, dtype=dtype, device="cuda")      # expanded: refused before anything is allocated
+        q, k = one.expand(n, lq, m, d), one.expand(n, lk, mk, d)
+        with pytest.raises(RuntimeError, match=match):
+            query_attention(q, k, k)
+
+    refused("heads of the query.* 128 tokens .*31 - 1 bytes", 128, 1, 1 << 18, 1 << 18, 32)
+    refused("heads of the query.* 256 tokens .*31 - 1 bytes", 5000, 1, 1 << 17, 1, 32)
+    refused("heads of the key.* 128 tokens .*31 - 1 bytes", 1, 128, 1 << 18, 1 << 18, 32)
+    refused("heads of the query.* 64 tokens .*31 - 1 bytes", 64, 1, 1 << 17, 1, 121)      # copied to 128 channels
+    refused("heads of the query.* 256 tokens .*31 - 1 bytes", 256, 1, 1 << 16, 1, 32, F32)
+    # workgroups of 64 columns, backward if not forward
+    refused("24 - 1 pieces of 64", 65, 1, 8, 1, 128, n=1 << 20)
+
+
+def test_the_most_heads_that_are_taken():
+    from dcnv4_amd.functions import query_attention
+    n, m, d = 128, (1 << 18) - 1, 32
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, grad = (torch.empty(1, n, m, d, dtype=F16, device="cuda").normal_(generator=gen) for _ in range(4))
+    wanted = [t.requires_grad_() for t in (q, k, v)]
+    out = query_attention(q, k, v)
+    grads = torch.autograd.grad(out, wanted, grad)
+    ends = torch.tensor([0, 1, m // 2, m - 2, m - 1], device="cuda")
+    few = lambda t: t.detach()[:, :, ends].cpu()
+    want = oracle_attention.attention(few(q), few(k), few(v), few(grad), unit=UNIT[F16], tiny=TINY[F16])
+    for name, got in zip(("out", "grad_query", "grad_key", "grad_value"), (out, *grads)):
+        close(few(got), want[name], name)
+
+
+@pytest.mark.parametrize("dtype", (F16, F32), ids=IDS.get)
+def test_single_tokens_of_very_many_heads(dtype):
+    # one row: nothing lies behind it
+    from dcnv4_amd.functions import query_attention
+    m, d = (1 << 20) + 3, 32
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.empty(1, 1, m, d, dtype=dtype, device="cuda").normal_(generator=gen) for _ in range(3))
+    # v w (1 / w) for the only weight w: three roundings of fp32, which fp16 does not show
+    off = (query_attention(q, k, v).double() - v.double()).abs() / v.double().abs().clamp_min(1e-30)
+    assert off.max() <= (0 if dtype == F16 else 3 * 2.0 ** -24)
