@@ -1,5 +1,7 @@
 // What stands between the sampling layers of a deformable decoder: attention among queries and the normalised sum.  Checks, dense
 // rows where the kernels need them, allocation and autograd nodes.
+#include <ATen/autocast_mode.h>
+
 #include <cmath>
 #include <tuple>
 
@@ -459,12 +461,8 @@ bool norm_takes(const NormInputs &a) {
   return !a.weight.defined() || !a.bias.defined() || a.weight.scalar_type() == a.bias.scalar_type();
 }
 
-// add_layer_norm(input, residual, weight, bias, eps, wide, want_sum): the result or (result, sum), or None where it is not taken
-PyObject *py_add_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  Args a("add_layer_norm", args, n, 7);
-  const NormInputs in = norm_inputs(a);
-  const bool want_sum = a.integer() != 0;
+// The result or (result, sum), with its node; None where it is not taken.
+PyObject *norm_call(const NormInputs &in, bool want_sum) {
   if (observed() || !norm_takes(in)) Py_RETURN_NONE;
   NormOutputs o;
   {
@@ -481,6 +479,51 @@ PyObject *py_add_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
   if (!want_sum) return THPVariable_Wrap(std::move(o.out));
   return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(o.out)), THPVariable_Wrap(std::move(o.sum)));
+}
+
+// add_layer_norm(input, residual, weight, bias, eps, wide, want_sum)
+PyObject *py_add_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("add_layer_norm", args, n, 7);
+  const NormInputs in = norm_inputs(a);
+  return norm_call(in, a.integer() != 0);
+  END_HANDLE_TH_ERRORS
+}
+
+// Whether a call of the module is torch's layer norm over the last axis with its parameters, and nothing else.
+bool plain_norm(const Module &norm, int64_t width) {
+  if (global_module_hooks() || !norm.called_as(kLayerNorm)) return false;
+  PyObject *shape = norm.attribute("normalized_shape");
+  return shape != nullptr && PyTuple_CheckExact(shape) && PyTuple_GET_SIZE(shape) == 1 && PyLong_Check(PyTuple_GET_ITEM(shape, 0)) &&
+         PyLong_AsLongLong(PyTuple_GET_ITEM(shape, 0)) == width;
+}
+
+// add_layer_norm_of(norm, input, residual, want_sum): the same of a module, read and checked here (its parameters by attribute take as long as
+// all the rest of a small call does on the host)
+PyObject *py_add_layer_norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("add_layer_norm_of", args + 1, n - 1, 3);
+  const Module norm(args[0]);
+  NormInputs in;
+  in.x = a.tensor();
+  in.residual = a.optional_tensor();
+  const bool want_sum = a.integer() != 0;
+  if (in.x.dim() < 1 || !plain_norm(norm, in.x.size(-1))) Py_RETURN_NONE;
+  in.weight = norm.parameter("weight");
+  in.bias = norm.parameter("bias");
+  const double eps = norm.real("eps", NAN);
+  if (std::isnan(eps)) Py_RETURN_NONE;      // a number of another class, which Python reads
+  in.eps = (float)eps;
+  in.wide = at::autocast::is_autocast_enabled(at::kCUDA);
+  return norm_call(in, want_sum);
+  END_HANDLE_TH_ERRORS
+}
+
+// plain_layer_norm(norm, width)
+PyObject *py_plain_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Args a("plain_layer_norm", args + 1, n - 1, 1);
+  return PyBool_FromLong(plain_norm(Module(args[0]), a.integer()));
   END_HANDLE_TH_ERRORS
 }
 
@@ -518,6 +561,8 @@ PyMethodDef decoder_methods[] = {FASTCALL("query_attention", py_query_attention)
                                  FASTCALL("query_attention_forward", py_query_attention_forward),
                                  FASTCALL("query_attention_backward", py_query_attention_backward),
                                  FASTCALL("add_layer_norm", py_add_layer_norm),
+                                 FASTCALL("add_layer_norm_of", py_add_layer_norm_of),
+                                 FASTCALL("plain_layer_norm", py_plain_layer_norm),
                                  FASTCALL("add_layer_norm_forward", py_add_layer_norm_forward),
                                  FASTCALL("add_layer_norm_backward", py_add_layer_norm_backward),
                                  {nullptr, nullptr, 0, nullptr}};

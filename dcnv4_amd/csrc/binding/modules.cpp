@@ -71,6 +71,14 @@ bool Module::computes(ModuleKind kind) const {
   return true;
 }
 
+bool Module::called_as(ModuleKind kind) const {
+  const Kind &k = g_kinds[kind];
+  if (o_ == nullptr || k.type == nullptr || !PyType_IsSubtype(Py_TYPE(o_), k.type)) return false;
+  for (int i = 0; i < kParts; ++i)
+    if (_PyType_Lookup(Py_TYPE(o_), name_object(kMethods[i])) != k.methods[i]) return false;
+  return !hooked();
+}
+
 Module Module::child(const char *name) const {
   PyObject *c = o_ != nullptr ? item(item(dict_of(o_), "_modules"), name) : nullptr;
   return Module(c == Py_None ? nullptr : c);

@@ -25,6 +25,7 @@ class Module {
   bool truth(const char *name, bool otherwise) const;
   bool is(ModuleKind kind) const;                             // exactly that class, its methods as they were registered
   bool computes(ModuleKind kind) const;                       // that class or a subclass that overrides no part of its forward
+  bool called_as(ModuleKind kind) const;                      // that class or a subclass, called with that class's forward and no hooks
   bool hooked() const;                                        // a hook or replaced method that a direct call of the kernels would miss
 
  private:

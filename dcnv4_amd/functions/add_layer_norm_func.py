@@ -2,8 +2,8 @@
 backward; the sum is not rounded before it is normalised.
 
 Runs on the library's kernels for rows of up to 8192 channels of any layout whose channels are dense, of any mix of float32 with
-one 16-bit type; otherwise (other types, CPU tensors, a norm over several axes) the expression is left to torch's own operators
-and autograd.
+one 16-bit type; otherwise (other types, CPU tensors, a norm over several axes; a norm with hooks or a forward of its own, which run) the
+expression is left to torch's own operators and autograd.
 """
 import torch
 from torch.autograd import Function
@@ -43,7 +43,7 @@ class AddLayerNormFunction(Function):
 
 
 def _fusable(x, residual, norm):
-    if not x.is_cuda or x.dim() < 1 or tuple(norm.normalized_shape) != (x.shape[-1],) or not 1 <= x.shape[-1] <= _MAX_CHANNELS:
+    if not x.is_cuda or not 1 <= x.shape[-1] <= _MAX_CHANNELS:
         return False
     tensors = [t for t in (x, residual, norm.weight, norm.bias) if t is not None]
     halves = {t.dtype for t in tensors if t.dtype != torch.float32}
@@ -59,13 +59,11 @@ def add_layer_norm(x, residual, norm, return_sum=False):
     wider type of the two, float32 under autocast as torch's own layer norm there.  With ``return_sum`` also the sum, in the wider type:
     ``(result, x + residual)``, the stream of a pre-norm network.  The backward reads x and residual again: neither is to be changed in
     place before it."""
-    weight, bias, wide = norm.weight, norm.bias, torch.is_autocast_enabled()
-    if weight is not None or tuple(norm.normalized_shape) == (x.shape[-1],):      # (the weight says as much)
-        output = _native.add_layer_norm(x, residual, weight, bias, norm.eps, wide, return_sum)
-        if output is not None:
-            return output
-    if not _fusable(x, residual, norm):
-        total = x if residual is None else x + residual
-        out = norm(total)
-        return (out, total) if return_sum else out
-    return AddLayerNormFunction.apply(x, residual, weight, bias, norm.eps, wide, bool(return_sum))
+    output = _native.add_layer_norm_of(norm, x, residual, return_sum)
+    if output is not None:
+        return output
+    if x.dim() and _native.plain_layer_norm(norm, x.shape[-1]) and _fusable(x, residual, norm):
+        return AddLayerNormFunction.apply(x, residual, norm.weight, norm.bias, norm.eps, torch.is_autocast_enabled(), bool(return_sum))
+    total = x if residual is None else x + residual
+    out = norm(total)
+    return (out, total) if return_sum else out

@@ -51,3 +51,61 @@ def test_single_tokens_of_very_many_heads(dtype):
     # v w (1 / w) for the only weight w: three roundings of fp32, which fp16 does not show
     off = (query_attention(q, k, v).double() - v.double()).abs() / v.double().abs().clamp_min(1e-30)
     assert off.max() <= (0 if dtype == F16 else 3 * 2.0 ** -24)
+
+
+class Doubled(torch.nn.LayerNorm):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class Named(torch.nn.LayerNorm):
+    """A subclass that leaves the forward as it is."""
+
+
+def norm_inputs(width=64):
+    gen = torch.Generator().manual_seed(3)
+    return [torch.randn(5, 7, width, generator=gen).cuda() for _ in range(3)]
+
+
+def seen_by(norm, register):
+    """What a hook that `register` puts on the norm sees of a call and its backward."""
+    from dcnv4_amd.functions import add_layer_norm
+    x, r, grad = norm_inputs()
+    seen = []
+    handle = register(lambda *args: seen.append(args))
+    try:
+        out = add_layer_norm(x.requires_grad_(), r, norm)
+        out.backward(grad)
+    finally:
+        handle.remove()
+    assert (out - torch.nn.functional.layer_norm(x + r, (64,), norm.weight, norm.bias, norm.eps)).abs().max() < 1e-5
+    return seen
+
+
+def test_hooks_of_a_norm_run():
+    norm = torch.nn.LayerNorm(64).cuda()
+    module = torch.nn.modules.module
+    for register in (norm.register_forward_hook, norm.register_forward_pre_hook, norm.register_full_backward_hook, norm.register_full_backward_pre_hook,
+                     module.register_module_forward_hook, module.register_module_forward_pre_hook):
+        assert len(seen_by(norm, register)) == 1, register
+
+
+def test_a_norms_own_forward_runs():
+    from dcnv4_amd.functions import add_layer_norm
+    x, r, _ = norm_inputs()
+    norm = Doubled(64).cuda()
+    out, total = add_layer_norm(x, r, norm, return_sum=True)
+    assert torch.equal(out, norm(x + r)) and torch.equal(total, x + r)
+    norm = torch.nn.LayerNorm(64).cuda()
+    norm.forward = lambda x: x + 1
+    assert torch.equal(add_layer_norm(x, r, norm), x + r + 1)
+    assert torch.equal(add_layer_norm(x, r, torch.nn.Identity()), x + r)
+    rms = torch.nn.RMSNorm(64).cuda()
+    assert torch.equal(add_layer_norm(x, r, rms), rms(x + r))
+
+
+def test_a_subclass_that_leaves_the_forward_as_it_is_takes_the_kernels():
+    from dcnv4_amd.functions import add_layer_norm
+    x, r, _ = norm_inputs()
+    out = add_layer_norm(x.requires_grad_(), r, Named(64).cuda())
+    assert out.grad_fn.name() == "AddLayerNormFunctionBackward"
