@@ -2,8 +2,8 @@
 (classification/models/flash_intern_image.py:425-440), as one kernel instead of the framework's three.
 
 Forward and backward run on the library's kernels whenever the tensors allow it (one floating dtype for activations
-and parameters, contiguous, channel count a whole number of 16-byte vectors, no autocast in force); otherwise the
-expression is left to torch's own operators and autograd.
+and parameters, contiguous, channel count a whole number of 16-byte vectors, no autocast in force, a norm without hooks or a
+forward of its own); otherwise the expression is left to torch's own operators and autograd.
 """
 import torch
 from torch.autograd import Function
@@ -47,7 +47,7 @@ def _fusable(y, residual, weight, bias, gamma):
 
 def layer_norm_residual(y, norm, gamma=None, residual=None):
     """``residual + gamma * norm(y)`` for an ``nn.LayerNorm`` over the last axis; ``gamma`` a per-channel tensor or None."""
-    if norm.weight is None or norm.bias is None or tuple(norm.normalized_shape) != (y.shape[-1],) or \
+    if not ext._native.plain_layer_norm(norm, y.shape[-1]) or norm.weight is None or norm.bias is None or \
             not _fusable(y, residual, norm.weight, norm.bias, gamma):
         out = norm(y)
         if gamma is not None:

@@ -109,3 +109,33 @@ def test_a_subclass_that_leaves_the_forward_as_it_is_takes_the_kernels():
     x, r, _ = norm_inputs()
     out = add_layer_norm(x.requires_grad_(), r, Named(64).cuda())
     assert out.grad_fn.name() == "AddLayerNormFunctionBackward"
+
+
+def test_a_block_tails_norm_runs_its_hooks_and_its_own_forward():
+    from dcnv4_amd.functions import layer_norm_residual
+    x, r, _ = norm_inputs()
+    gamma = torch.rand(64, device="cuda")
+    norm, seen = torch.nn.LayerNorm(64).cuda(), []
+    plain = layer_norm_residual(x, norm, gamma, r)
+    handle = norm.register_forward_hook(lambda *args: seen.append(args))
+    hooked = layer_norm_residual(x, norm, gamma, r)
+    handle.remove()
+    assert len(seen) == 1 and (hooked - plain).abs().max() < 1e-5
+    doubled = Doubled(64).cuda()
+    assert torch.equal(layer_norm_residual(x, doubled, gamma, r), r + gamma * doubled(x))
+    assert torch.equal(layer_norm_residual(x, torch.nn.Identity()), x)
+    assert layer_norm_residual(x.requires_grad_(), Named(64).cuda()).grad_fn.name() == "LayerNormResidualFunctionBackward"
+
+
+def test_hooks_inside_a_layer_run():
+    from dcnv4_amd.models.flash_intern_image import InternImageLayer
+    layer = InternImageLayer(channels=64, groups=4, layer_scale=1.0).cuda().eval()
+    norms = [m for m in layer.modules() if isinstance(m, torch.nn.LayerNorm)]
+    x, seen = torch.randn(1, 64, 64, device="cuda"), []
+    with torch.no_grad():
+        plain = layer(x, (8, 8))
+        handles = [m.register_forward_hook(lambda *args: seen.append(args)) for m in norms]
+        hooked = layer(x, (8, 8))
+    for h in handles:
+        h.remove()
+    assert norms and len(seen) == len(norms) and (hooked - plain).abs().max() < 1e-4
