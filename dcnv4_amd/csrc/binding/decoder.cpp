@@ -174,8 +174,7 @@ std::array<Tensor, 4> attn_backward(const AttnInputs &a, const AttnOutputs &foun
 }
 
 struct QueryAttentionBackward final : torch::autograd::Node {
-  SavedVariable q, k, v, q_segments, k_segments, q_points, k_points, slopes, out;
-  Tensor rest, lse;
+  SavedVariable q, k, v, q_segments, k_segments, q_points, k_points, slopes, out, rest, lse;      // all that hooks for saved tensors may pack
   float scale, cap;
 
   explicit QueryAttentionBackward(const AttnInputs &a)
@@ -183,8 +182,7 @@ struct QueryAttentionBackward final : torch::autograd::Node {
         q_points(a.q_points, false), k_points(a.k_points, false), slopes(a.slopes, false), scale(a.scale), cap(a.cap) {}
   std::string name() const override { return "QueryAttentionFunctionBackward"; }
   void release_variables() override {
-    for (SavedVariable *s : {&q, &k, &v, &q_segments, &k_segments, &q_points, &k_points, &slopes, &out}) s->reset_data();
-    rest = lse = Tensor();
+    for (SavedVariable *s : {&q, &k, &v, &q_segments, &k_segments, &q_points, &k_points, &slopes, &out, &rest, &lse}) s->reset_data();
   }
   variable_list apply(variable_list &&grads) override {
     if (!grads[0].defined()) return variable_list(4);
@@ -195,7 +193,7 @@ struct QueryAttentionBackward final : torch::autograd::Node {
                             slopes.unpack(), scale, cap};
       const Tensor o = out.unpack(shared_from_this());
       Tensor g = grads[0]._is_zerotensor() ? at::zeros(grads[0].sizes(), grads[0].options()) : grads[0];
-      got = attn_backward(a, {o, rest, lse}, g, {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2),
+      got = attn_backward(a, {o, rest.unpack(), lse.unpack()}, g, {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2),
                                          task_should_compute_output(3)});
     }
     return once_differentiable({got[0], got[1], got[2], got[3]});
@@ -235,8 +233,8 @@ PyObject *py_query_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
       node->set_next_edges(torch::autograd::collect_next_edges(in.q, in.k, in.v, in.slopes));
       record(node, out);
       node->out = SavedVariable(out, true);
-      node->rest = found.rest;
-      node->lse = found.lse;
+      node->rest = SavedVariable(found.rest, false);
+      node->lse = SavedVariable(found.lse, false);
     }
   }
   return THPVariable_Wrap(std::move(out));
@@ -391,8 +389,7 @@ std::array<Tensor, 4> norm_backward(const NormInputs &a, const Tensor &stats, co
 
 // The summands are kept, not the sum: rounded to 16 bits it would show in the gradient of weight.
 struct AddLayerNormBackward final : torch::autograd::Node {
-  SavedVariable x, residual, weight, bias;
-  Tensor stats;
+  SavedVariable x, residual, weight, bias, stats;
   float eps;
   bool wide, has_residual;
   at::ScalarType x_dtype, residual_dtype;
@@ -402,8 +399,7 @@ struct AddLayerNormBackward final : torch::autograd::Node {
         has_residual(a.residual.defined()), x_dtype(a.x.scalar_type()), residual_dtype(has_residual ? a.residual.scalar_type() : x_dtype) {}
   std::string name() const override { return "AddLayerNormFunctionBackward"; }
   void release_variables() override {
-    for (SavedVariable *s : {&x, &residual, &weight, &bias}) s->reset_data();
-    stats = Tensor();
+    for (SavedVariable *s : {&x, &residual, &weight, &bias, &stats}) s->reset_data();
   }
   variable_list apply(variable_list &&grads) override {
     const Tensor around = grads.size() > 1 ? grads[1] : Tensor();
@@ -423,7 +419,7 @@ struct AddLayerNormBackward final : torch::autograd::Node {
         a.bias = bias.unpack();
         a.eps = eps;
         a.wide = wide;
-        got = norm_backward(a, stats, dense(grads[0]), dense(around),
+        got = norm_backward(a, stats.unpack(), dense(grads[0]), dense(around),
                             {task_should_compute_output(0), has_residual && task_should_compute_output(1), task_should_compute_output(2),
                              task_should_compute_output(3)});
       }
@@ -474,7 +470,7 @@ PyObject *norm_call(const NormInputs &in, bool want_sum) {
       node->set_next_edges(torch::autograd::collect_next_edges(in.x, in.residual, in.weight, in.bias));
       record(node, o.out);
       if (want_sum) record(node, o.sum);
-      node->stats = o.stats;
+      node->stats = SavedVariable(o.stats, false);
     }
   }
   if (!want_sum) return THPVariable_Wrap(std::move(o.out));

@@ -139,3 +139,70 @@ def test_hooks_inside_a_layer_run():
     for h in handles:
         h.remove()
     assert norms and len(seen) == len(norms) and (hooked - plain).abs().max() < 1e-4
+
+
+def attention_inputs(dtype):
+    from tests.test_gpu_query_attention import inputs, leaves, on_gpu
+    t = on_gpu(inputs(2, 500, 500, 4, 4, 32, dtype, mask="documents", distance=True, seed=51))
+    return t, leaves(t)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+def test_all_that_attention_keeps_passes_through_hooks_for_saved_tensors(dtype):
+    from tests.test_gpu_query_attention import call
+    t, wanted = attention_inputs(dtype)
+    plain = call(t)
+    plain_grads = torch.autograd.grad(plain, wanted, t["grad"])
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        out = call(t)
+    # what stays on the GPU is the result
+    assert torch.cuda.memory_allocated() - before <= out.numel() * out.element_size() + 512
+    assert torch.equal(out, plain)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, wanted, t["grad"]), plain_grads))
+
+
+@pytest.mark.parametrize("dtype", (F32, F16), ids=IDS.get)
+def test_all_that_a_normalised_sum_keeps_passes_through_hooks_for_saved_tensors(dtype):
+    from dcnv4_amd.functions import add_layer_norm
+    gen = torch.Generator().manual_seed(4)
+    x, r, grad = (torch.randn(20000, 16, generator=gen).to(dtype).cuda() for _ in range(3))
+    norm = torch.nn.LayerNorm(16).cuda().to(dtype)
+    wanted = [x.requires_grad_(), r.requires_grad_(), norm.weight, norm.bias]
+    plain = add_layer_norm(x, r, norm)
+    plain_grads = torch.autograd.grad(plain, wanted, grad)
+    before = torch.cuda.memory_allocated()
+    with torch.autograd.graph.save_on_cpu():
+        out = add_layer_norm(x, r, norm)
+    assert torch.cuda.memory_allocated() - before <= out.numel() * out.element_size() + 512
+    assert torch.equal(out, plain)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, wanted, grad), plain_grads))
+
+
+def test_operators_under_checkpointing():
+    from torch.utils.checkpoint import checkpoint
+    from dcnv4_amd.functions import add_layer_norm
+    from tests.test_gpu_query_attention import call
+    t, wanted = attention_inputs(F16)
+    norm = torch.nn.LayerNorm(32).cuda()
+    wanted.append(norm.weight)
+
+    def step(query):
+        return add_layer_norm(call(dict(t, q=query)), query, norm)
+
+    plain = step(t["q"])
+    out = checkpoint(step, t["q"], use_reentrant=False)
+    assert torch.equal(out, plain)
+    for a, b in zip(torch.autograd.grad(out, wanted, t["grad"].to(out.dtype)), torch.autograd.grad(plain, wanted, t["grad"].to(out.dtype))):
+        assert torch.equal(a, b)
+
+
+def test_a_second_backward_of_what_is_kept_and_of_what_is_freed():
+    from tests.test_gpu_query_attention import call
+    t, wanted = attention_inputs(F16)
+    out = call(t)
+    first = torch.autograd.grad(out, wanted, t["grad"], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(out, wanted, t["grad"])))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, wanted, t["grad"])
