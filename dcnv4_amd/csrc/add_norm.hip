@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kMostThreads) add_norm_backward_kernel(const A
       Access<Out, G>::decode(next_g[n], a[n]);
       Access<Sum, G>::decode(next_s[n], around[n]);
     }
-    const float rstd = next_stats.y, shift = -next_stats.x * rstd;
+    const float mean = next_stats.x, rstd = next_stats.y;
     request(row + teams);
     float sums[2] = {0.f, 0.f};
     // beyond the width and the rows the gradients are zeros, and so is all that is added up
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kMostThreads) add_norm_backward_kernel(const A
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int c = 0; c < G; ++c) {
-        z[n][c] = fmaf(z[n][c], rstd, shift);
+        z[n][c] = (z[n][c] - mean) * rstd;      // as the forward: z rstd - mean rstd would lose what is small beside the mean
         dw[n][c] = fmaf(a[n][c], z[n][c], dw[n][c]);
         db[n][c] += a[n][c];
         a[n][c] *= w[n][c];

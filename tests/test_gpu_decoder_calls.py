@@ -206,3 +206,23 @@ def test_a_second_backward_of_what_is_kept_and_of_what_is_freed():
     assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(out, wanted, t["grad"])))
     with pytest.raises(RuntimeError, match="second time"):
         torch.autograd.grad(out, wanted, t["grad"])
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+def test_rows_without_deviation_do_not_show_in_the_weights_gradient(dtype):
+    # 64 equal numbers have an exact mean: xhat is zero, forward and backward, whatever their size beside the deviation
+    from dcnv4_amd.functions import add_layer_norm
+    gen = torch.Generator().manual_seed(5)
+    norm = torch.nn.LayerNorm(64).cuda()
+    x = (torch.randint(1, 200, (300, 1), generator=gen) * 3.0).expand(300, 64).to(dtype).cuda().requires_grad_()
+    r = torch.ones(300, 64, dtype=dtype, device="cuda")
+    out = add_layer_norm(x, r, norm)
+    grad = torch.randn(300, 64, generator=gen).to(out.dtype).cuda()
+    assert torch.equal(out, norm.bias.to(out.dtype).expand(300, 64))
+    grad_weight, grad_x = torch.autograd.grad(out, (norm.weight, x), grad)
+    assert not grad_weight.any()
+    # and the summands' are rstd (g - mean(g)): a rounding of the type, and a few of fp32 of sums of 64
+    g = grad.double()
+    want = (g - g.mean(-1, keepdim=True)) * norm.eps ** -0.5
+    off = UNIT[dtype] * want.abs() + 2.0 ** -20 * norm.eps ** -0.5 * (g.abs() + g.abs().mean(-1, keepdim=True))
+    assert ((grad_x.double() - want).abs() <= off).all()
