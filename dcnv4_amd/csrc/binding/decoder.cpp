@@ -13,7 +13,6 @@ namespace dcn::binding {
 namespace {
 
 constexpr int64_t kIntMax = 0x7fffffff;
-constexpr float kFloatMax = 3.402823466e38f;
 
 // ---------------------------------------------------------------- attention among queries
 struct AttnInputs {
@@ -66,8 +65,10 @@ AttnShape attn_check(const AttnInputs &a) {
   const int64_t piece = row_bytes > 128 ? 64 : 128;
   if (s.batch * s.heads * ((s.nq + piece - 1) / piece) >= 1 << 24 || s.batch * s.kv_heads * ((s.nk + piece - 1) / piece) >= 1 << 24)
     raise_runtime("more than 2^24 - 1 pieces of %lld queries or keys of a head", (long long)piece);
-  if (!(std::fabs(a.scale) < kFloatMax)) raise_runtime("scale must be finite");
+  // (the kernels multiply both by a number below three: what passes fp32 would be NaN where a product is zero)
+  if (!(std::fabs(a.scale) <= 1e30f)) raise_runtime("scale must be between -1e30 and 1e30");
   if (a.cap != 0.f && !(a.cap >= 1e-30f && a.cap <= 1e30f)) raise_runtime("cap must be zero (none) or between 1e-30 and 1e30");
+  if (a.cap != 0.f && std::fabs(a.scale) > 1.000001e30 * a.cap) raise_runtime("scale may be up to 1e30 times cap");
   if (a.q_segments.defined()) {
     check_beside(a.q_segments, "segments", a.q, at::kInt, {s.batch, s.nq});
     if (!a.k_segments.defined()) raise_runtime("segments without key_segments");

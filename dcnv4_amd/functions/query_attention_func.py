@@ -57,8 +57,8 @@ def query_attention(query, key, value, *, scale=None, cap=0.0, segments=None, ke
     key head) and D up to 128, all float32, float16 or bfloat16; views of a fused projection are read as they lie.  ``segments``
     (N, Lq) and ``key_segments`` (N, Lk) int32: for self-attention one is enough; ``key_segments`` alone (0 and -1: padded keys)
     counts all queries as 0.  ``positions`` (N, Lq, 2), ``key_positions`` (N, Lk, 2; the queries' own if left out) and ``slopes``
-    (M,) float32.  Gradients reach query, key, value and slopes.  Under autocast the first three are cast to its type.
-    Returns (N, Lq, M, D)."""
+    (M,) float32.  ``scale`` is at most 1e30 in size, ``cap`` 0 or 1e-30 to 1e30, the first at most 1e30 times the second.  Gradients
+    reach query, key, value and slopes.  Under autocast the first three are cast to its type.  Returns (N, Lq, M, D)."""
     for points in (positions, key_positions):
         if points is not None and points.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("query_attention has no gradient for positions: detach them")

@@ -67,3 +67,16 @@ def test_slopes_of_any_size(scale, dtype):
     t["k_points"][:, :45] = t["q_points"][:, 45:]          # some of the points meet
     t["q_points"][:, :45] = t["k_points"][:, :45]
     check(t, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+def test_scales_to_the_end_of_their_range(dtype):
+    from dcnv4_amd.functions import query_attention
+    q, k = torch.zeros(1, 5, 2, 16, dtype=dtype, device="cuda"), torch.ones(1, 8, 2, 16, dtype=dtype, device="cuda")
+    v = torch.ones(1, 8, 2, 16, dtype=dtype, device="cuda")
+    # products of zero: all keys weigh the same, and the eight of them add up to one
+    for scale, cap in ((1e30, 0.0), (-1e30, 0.0), (1.0, 1e-30), (1e30, 1.0), (-1e30, 1e30)):
+        assert torch.equal(query_attention(q, k, v, scale=scale, cap=cap), torch.ones_like(q)), (scale, cap)
+    for scale, cap, match in ((3e38, 0.0, "scale must be between"), (-1.1e30, 0.0, "scale must be between"), (2.0, 1e-30, "times cap"), (1e30, 0.5, "times cap")):
+        with pytest.raises(RuntimeError, match=match):
+            query_attention(q, k, v, scale=scale, cap=cap)
