@@ -15,7 +15,8 @@ number is not negative and j's is the same or 0:
   * padding (any negative number), which nothing sees and which sees nothing.
 
 A row that sees nothing is zeros and sends no gradient.  What a row does not see has no influence on it whatever it holds,
-infinities and NaN too.
+infinities and NaN too.  One that it does see in a value takes its channel of the head's result with it, or the head's whole result of that
+row: which of the two is a matter of how the keys fall into tiles.  Other heads, and rows that do not see it, are left as they are.
 """
 import torch
 from torch.autograd import Function

@@ -80,3 +80,18 @@ def test_scales_to_the_end_of_their_range(dtype):
     for scale, cap, match in ((3e38, 0.0, "scale must be between"), (-1.1e30, 0.0, "scale must be between"), (2.0, 1e-30, "times cap"), (1e30, 0.5, "times cap")):
         with pytest.raises(RuntimeError, match=match):
             query_attention(q, k, v, scale=scale, cap=cap)
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("bad", (float("inf"), float("nan")))
+@pytest.mark.parametrize("lq,lk,where", [(40, 300, 3), (40, 300, 299), (700, 130, 129), (1, 20, 19), (2, 5001, 5000)])
+def test_an_infinite_value_that_all_see_stays_in_its_head(lq, lk, where, bad, dtype):
+    t = on_gpu(inputs(1, lq, lk, 2, 2, 32, dtype, seed=46, spread=0.3))
+    for train in (False, True):
+        wanted = leaves(t) if train else []
+        clean = call(t).detach()
+        v = t["v"].detach().clone()
+        v[0, where, 1, 5] = bad
+        out = call(dict(t, v=v.requires_grad_(train))).detach()
+        assert not torch.isfinite(out[:, :, 1, 5]).any()
+        assert torch.equal(out[:, :, 0], clean[:, :, 0])
