@@ -11,8 +11,9 @@
 //
 // Rows that all start on 16 bytes go in vectors of eight elements.  Others (an odd width, an odd offset) go element by element, neighbours
 // in neighbouring lanes: a 16-byte access that crosses its alignment costs twice (100000 x 1023, 16 bits, forward 283 us and backward 589
-// in unaligned vectors, 195 and 251 so; 1024 channels 147 and 222).  The backward reads four tensors for the one it writes, which
-// memory gives at some 4.5 TB/s, a copy 6.2; loads two rows ahead were slower (401408 x 112: 112 us for 98).
+// in unaligned vectors, 195 and 251 so; 1024 channels 147 and 222, all on one machine; on another 164 and 233, and 121 and 179).  The backward
+// reads up to four tensors for the one it writes: 4.5 to 4.7 TB/s of the 5.0 to 5.3 that a plain stream of that mix reaches; loads two rows ahead
+// were slower (401408 x 112: 112 us for 98).
 //
 // The parameters' gradients are summed in registers down a workgroup's slab, over its teams through LDS, and over the workgroups by a
 // second kernel, always in the same order.
