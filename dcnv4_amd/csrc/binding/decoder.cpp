@@ -520,7 +520,9 @@ PyObject *py_add_layer_norm_of(PyObject *, PyObject *const *args, Py_ssize_t n) 
 PyObject *py_plain_layer_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Args a("plain_layer_norm", args + 1, n - 1, 1);
-  return PyBool_FromLong(plain_norm(Module(args[0]), a.integer()));
+  const long long width = PyLong_AsLongLong(args[1]);
+  if (width == -1 && PyErr_Occurred()) throw python_error();
+  return PyBool_FromLong(plain_norm(Module(args[0]), width));
   END_HANDLE_TH_ERRORS
 }
 
