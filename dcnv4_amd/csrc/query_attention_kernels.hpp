@@ -644,6 +644,15 @@ struct Split {
   float *part, *stats;                // [chunk][batch][query][head][width], [..][2]: unnormalised sums; maximum and sum
 };
 
+// What the backward forms a row's weights from again: infinite, so zeros, where it sees nothing.  A weight is then off by half a last bit of the
+// logarithm and of its score: 1e-4 of it for scores of 1000 (in units of exp2), some hundredths at 2^20.  Beyond that what comes out has lost its
+// size, of a single key's weight too (2^8 for one at 1e8): no number rather than a wrong one.
+template <typename Tag>
+__device__ __forceinline__ float row_logarithm(float top, float sum) {
+  if (sum == 0.f) return kInf;
+  return fabsf(top) > 0x1p20f ? __builtin_nanf("") : top - kForwardShift<Tag> + __builtin_amdgcn_logf(sum);
+}
+
 // TRAIN: a backward follows (16-bit types; fp32 ones have nothing to round).
 template <typename S, bool TRAIN>
 __global__ void __launch_bounds__(S::kThreads, S::kForwardWaves) attn_forward_kernel(const AttnLaunch p, const Split split) {
@@ -872,7 +881,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kForwardWaves) attn_forward_ke
     if (g != 0 || row_wave != 0) continue;
     if (split_rows) reinterpret_cast<f32x2 *>(split.stats)[part_row] = f32x2{top[f], sum[f]};
     else if (p.lse != nullptr)
-      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = sum[f] == 0.f ? kInf : top[f] - kForwardShift<Tag> + __builtin_amdgcn_logf(sum[f]);
+      p.lse[((size_t)at.b * p.heads + at.head) * p.nq + i] = row_logarithm<Tag>(top[f], sum[f]);
   }
 }
 
@@ -909,7 +918,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnLaunc
   if (p.out_rest != nullptr) store4<Tag>(p.out_rest, row * p.width + column, rounded_off<Tag>(acc));
   if (p.lse != nullptr && column == 0) {
     const long long head = row % p.heads, i = row / p.heads % p.nq, b = row / p.heads / p.nq;
-    p.lse[(b * p.heads + head) * p.nq + i] = sum == 0.f ? kInf : top - kForwardShift<Tag> + __builtin_amdgcn_logf(sum);
+    p.lse[(b * p.heads + head) * p.nq + i] = row_logarithm<Tag>(top, sum);
   }
 }
 

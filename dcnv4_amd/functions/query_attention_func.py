@@ -17,6 +17,9 @@ number is not negative and j's is the same or 0:
 A row that sees nothing is zeros and sends no gradient.  What a row does not see has no influence on it whatever it holds,
 infinities and NaN too.  One that it does see in a value takes its channel of the head's result with it, or the head's whole result of that
 row: which of the two is a matter of how the keys fall into tiles.  Other heads, and rows that do not see it, are left as they are.
+
+Gradients form the weights again from the logarithm of a row's sum, in fp32: they are off by 2^-23 of the size of the row's largest score, relatively.
+A row whose largest score passes 7e5 in size, as where even the nearest key is that far away times the slope, has its result, and NaN as gradients.
 """
 import torch
 from torch.autograd import Function

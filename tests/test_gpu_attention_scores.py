@@ -95,3 +95,26 @@ def test_an_infinite_value_that_all_see_stays_in_its_head(lq, lk, where, bad, dt
         out = call(dict(t, v=v.requires_grad_(train))).detach()
         assert not torch.isfinite(out[:, :, 1, 5]).any()
         assert torch.equal(out[:, :, 0], clean[:, :, 0])
+
+
+@pytest.mark.parametrize("dtype", (F32, F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("lq,lk", [(3, 1), (40, 300), (2, 5001)])
+@pytest.mark.parametrize("cap", (0.0, 50.0))
+def test_gradients_of_rows_that_are_far_from_all_keys(cap, lq, lk, dtype):
+    t = inputs(2, lq, lk, 2, 2, 32, dtype, distance=True, seed=47)
+    t["q_points"][:], t["k_points"][:] = 0.0, 1.0
+    t["q_points"][:, 0] = 1.0          # where all keys are
+    t["slopes"] = torch.tensor([30.0, 1e4])
+    check(t, cap=cap)
+    # the second head's queries, but for the first, are a million and a half away
+    t["slopes"] = torch.tensor([30.0, 1.1e6])
+    gpu = on_gpu(t)
+    wanted = leaves(gpu)
+    out = call(gpu, cap=cap)
+    near = call(dict(gpu, slopes=torch.tensor([30.0, 0.0], device="cuda")), cap=cap)
+    # distances that are all alike do not weigh, but for the last bits that scores of their size leave of the products
+    assert torch.isfinite(out).all() and torch.equal(out[:, 0, 1], near[:, 0, 1])
+    grad_query, grad_key, grad_value, grad_slopes = torch.autograd.grad(out, wanted, gpu["grad"])
+    assert torch.isnan(grad_query[:, 1:, 1]).all() and torch.isnan(grad_key[:, :, 1]).all() and torch.isnan(grad_value[:, :, 1]).all()
+    assert all(torch.isfinite(g).all() for g in (grad_query[:, :, 0], grad_query[:, 0], grad_key[:, :, 0], grad_value[:, :, 0], grad_slopes[0]))
+    assert torch.isnan(grad_slopes[1])
