@@ -53,12 +53,15 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32, kWave);
 }
 
-// A kernel's shape.  W: the width, zeros behind the tensors' own; RT: rows of a tile; RW: waves that share the columns and divide
+// What goes into a kernel's scores: a cap, distances or a factor that is not positive; the products alone; a cap above kQuickCap, in 16-bit types.
+enum ScoreKind { kAnyScores, kPlainScores, kHighCap };
+// A kernel's shape.  KIND: a ScoreKind; W: the width, zeros behind the tensors' own; RT: rows of a tile; RW: waves that share the columns and divide
 // a tile's rows, the others divide the columns; CF: sixteens of columns a wave; WAVES: of a workgroup.
-template <typename Tag_, bool PLAIN_, int W_, int RT_, int RW_, int CF_, int WAVES_>
+template <typename Tag_, int KIND_, int W_, int RT_, int RW_, int CF_, int WAVES_>
 struct Shape {
   typedef Tag_ Tag;
-  static constexpr bool kPlain = PLAIN_;
+  static constexpr int kKind = KIND_;
+  static constexpr bool kPlain = KIND_ == kPlainScores;
   static constexpr int W = W_, RT = RT_, RW = RW_, CF = CF_, kWaves = WAVES_, kThreads = kWaves * kWave;
   static constexpr int kSlices = W * Tag::kBytes / 64, kWidthBlocks = W / 16;
   static constexpr int kColumnWaves = kWaves / RW, kColumns = 16 * CF * kColumnWaves;
@@ -75,7 +78,7 @@ struct Shape {
   static constexpr int kWavesPerSimd = W * Tag::kBytes > 256 ? 1 : 2;
   // narrow heads by 64 columns: three where that costs next to no scratch memory.  32 channels, bf16: forward of 32 heads, 2500 queries 92 -> 83
   // us, with distances 122 -> 112; dK and dV of bf16 96 -> 87 (fp16, with its scales a column, or distances: spills, 32 -> 40).  What is kept
-  // in scratch memory: 24 to 48 bytes a lane there, 60 in the 16-bit forward of 128 channels by 128 columns with caps or distances, 12 to 36 in
+  // in scratch memory: 20 to 44 bytes a lane there, 36 in the 16-bit forward of 128 channels by 128 columns with caps or distances, 12 to 36 in
   // fp16's dK and dV of 64 channels by 128 columns with them and by 32
   static constexpr bool kNarrow = W * Tag::kBytes <= 64 && RW == 2;
   static constexpr int kForwardWaves = kNarrow ? 3 : kWavesPerSimd, kGradKvWaves = kNarrow && kPlain && Tag::kCode == BF16::kCode ? 3 : kWavesPerSimd;
@@ -306,11 +309,11 @@ __device__ __forceinline__ void two_products(const char *first, const char *seco
 // ---------------------------------------------------------------- scores
 // 16-bit types form cap tanh(x / cap) as cap - 2 cap / (exp(2 x / cap) + 1), four instructions whose error is that of numbers of the cap's size:
 // at most 2^-20 cap (a last bit of exponential and reciprocal each, the sum's half), which the weights show.  At 256 that is half a rounding
-// of fp16's weights; higher caps take a form that is exact for small x / cap.
+// of fp16's weights; higher caps take a form that is exact for small x / cap, in kernels of their own: as a branch of the others it cost every
+// call with a cap 2 %.
 constexpr float kQuickCap = 256.f;
 // To a relative 2^-21: a series whose next term is 3e-7 at 1/4, and beyond it (1 - e) / (1 + e) with e = exp(-2 |x|), which loses no digits there.
-// fp32 results see the last bits, which tanhf has.  16-bit types do without its registers: kernels that keep some in scratch memory already
-// would keep a dozen more.
+// fp32 results see the last bits, which tanhf has; it takes more registers.
 template <typename Tag>
 __device__ __forceinline__ float exact_tanh(float x) {
   if constexpr (Tag::kBytes == 4) return tanhf(x);
@@ -320,11 +323,12 @@ __device__ __forceinline__ float exact_tanh(float x) {
 }
 // Scores go into exp2, so they are in units of its exponent.  Without cap and distance that is one factor, which rides along where
 // the maximum is taken off.
-template <bool PLAIN>
+template <int KIND>
 struct Scores {
   float tanh_scale, factor, slope;
-  bool bent, high, apart, scaled;      // there is a cap; one above kQuickCap; a distance; neither, but a factor that cannot ride along
-  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : bent(p.cap > 0.f), high(p.cap > kQuickCap), apart(p.slopes != nullptr) {
+  static constexpr bool high = KIND == kHighCap;
+  bool bent, apart, scaled;      // there is a cap; a distance; neither, but a factor that cannot ride along
+  __device__ __forceinline__ Scores(const AttnLaunch &p, int head) : bent(high || p.cap > 0.f), apart(p.slopes != nullptr) {
     tanh_scale = bent ? p.scale / p.cap : 0.f;
     factor = (bent ? p.cap : p.scale) * kLog2e;
     slope = apart ? p.slopes[head] * kLog2e : 0.f;
@@ -334,7 +338,7 @@ struct Scores {
 // Nothing but a positive factor: the products stand for the scores, in the order of their size.  Kernels of their own, which have
 // registers for more waves.
 template <>
-struct Scores<true> {
+struct Scores<kPlainScores> {
   float factor;
   static constexpr float tanh_scale = 0.f, slope = 0.f;
   static constexpr bool bent = false, high = false, apart = false, scaled = false;
@@ -350,11 +354,11 @@ __device__ __forceinline__ float distance(f32x2 a, f32x2 b) {
 // Scores of N blocks of 16 rows, from the products in s.  What a call has is the same for all lanes: a loop for each, not a question
 // for each score.  Forward; where `by_slope` says so the scores are left in units of the slope, `ratio` being the product's factor in them.
 // Positions are subtracted as they come, which is exact for near points, and in the backward too.
-template <typename Tag, bool PLAIN, int N, int CF, typename Points>
-__device__ __forceinline__ void finish_scores(const Scores<PLAIN> &scores, bool by_slope, float ratio, f32x4 (&s)[N][CF], const f32x2 (&point)[CF], Points point_of) {
+template <typename Tag, int KIND, int N, int CF, typename Points>
+__device__ __forceinline__ void finish_scores(const Scores<KIND> &scores, bool by_slope, float ratio, f32x4 (&s)[N][CF], const f32x2 (&point)[CF], Points point_of) {
   if (scores.bent) {
     const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
-    if (Tag::kBytes == 4 || scores.high) {
+    if constexpr (Tag::kBytes == 4 || Scores<KIND>::high) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -398,10 +402,10 @@ __device__ __forceinline__ void finish_scores(const Scores<PLAIN> &scores, bool 
 }
 // Backward: weights of 32 rows without what is not seen, from the products in s and the rows' or columns' logarithms; the distances,
 // and the tanh's derivative over kBendFactor.  seen(): masks s in place, before the exponential.
-template <typename Tag, bool PLAIN, int CF, typename Points, typename Lse, typename Seen>
-__device__ __forceinline__ void form_weights(const Scores<PLAIN> &scores, f32x4 (&s)[2][CF], f32x4 (&far)[2][CF], f32x4 (&bend)[2][CF], const f32x2 (&point)[CF],
+template <typename Tag, int KIND, int CF, typename Points, typename Lse, typename Seen>
+__device__ __forceinline__ void form_weights(const Scores<KIND> &scores, f32x4 (&s)[2][CF], f32x4 (&far)[2][CF], f32x4 (&bend)[2][CF], const f32x2 (&point)[CF],
                                              Points point_of, Lse lse, Seen seen) {
-  if constexpr (PLAIN) {
+  if constexpr (KIND == kPlainScores) {
     seen();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -413,7 +417,7 @@ __device__ __forceinline__ void form_weights(const Scores<PLAIN> &scores, f32x4 
   }
   if (scores.bent) {
     const float rate = scores.tanh_scale * (2.f * kLog2e), twice = -2.f * scores.factor;
-    if (Tag::kBytes == 4 || scores.high) {
+    if constexpr (Tag::kBytes == 4 || Scores<KIND>::high) {
       constexpr float bend0 = 1.f / kBendFactor<Tag>;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -666,11 +670,12 @@ __global__ void __launch_bounds__(S::kThreads, S::kForwardWaves) attn_forward_ke
   const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
   const int first = at.chunk * split.chunk_rows, last = min(p.nk, first + split.chunk_rows);
   const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
-  const Scores<S::kPlain> scores(p, at.head);
+  const Scores<S::kKind> scores(p, at.head);
   const bool masked = p.k_segments != nullptr;
   // without a cap the product's factor and the distance are one operation in units of a positive slope, which rides along where the
   // maximum is taken off; a slope within 2^20 of the factor, so that no score leaves the range of fp32 in its units.  (The ratio in a scalar
-  // register: 4 x 2500 queries of 8 heads of 32, bf16, with distances 119 us, 113 so; the slope in one as well, calls with a cap take 5 % longer.)
+  // register leaves others a vector register: 2 x 7744 queries of 8 heads of 64, bf16, with a cap and distances 873 us, 856 so; the slope in
+  // one as well, 5 % longer.)
   const float ratio = wave_uniform(scores.apart ? scores.factor / scores.slope : 0.f);
   const bool by_slope = scores.apart && !scores.bent && scores.slope > 0.f && fabsf(ratio) >= 0x1p-20f && fabsf(ratio) <= 0x1p20f;
   const float factor = S::kPlain ? scores.factor : (by_slope ? scores.slope : 1.f);
@@ -696,7 +701,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kForwardWaves) attn_forward_ke
   // goes through the products as well: delta, and the logarithm from which the weights are formed again, then belong to the weights
   // themselves (with delta of rounded ones dQ was off by 1.5 of its own roundings, with those of 1.4).  Without a backward the rounding stays:
   // results are off by 2.6e-4 to 2.8e-4 in fp16 and 2.2e-3 in bf16, root mean square, where one rounding of the result alone is 2.1e-4 and
-  // 1.7e-3, and the rests would cost half as much again (2 x 4096 tokens, 8 heads of 64, bf16: 100 us, with them 146).
+  // 1.7e-3, and the rests would cost half as much again (2 x 4096 tokens, 8 heads of 64, bf16: 100 us, with them 145).
   f32x4 acc[S::kWidthBlocks][S::CF], total[S::CF];
   float top[S::CF];
 #pragma unroll
@@ -751,7 +756,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kForwardWaves) attn_forward_ke
         for (int f = 0; f < S::CF; ++f) s[n][f] = mfma_64_bytes<Tag>(a[n & 1][sl], q[f][sl], s[n][f]);
     }
     const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block0 * 16 + 4 * g;
-    finish_scores<Tag, S::kPlain, S::kRowBlocks, S::CF>(scores, by_slope, ratio, s, point, [&](int n, int r) { return points[n * 16 + r]; });
+    finish_scores<Tag, S::kKind, S::kRowBlocks, S::CF>(scores, by_slope, ratio, s, point, [&](int n, int r) { return points[n * 16 + r]; });
     if (!every)
 #pragma unroll
       for (int n = 0; n < S::kRowBlocks; ++n) {
@@ -997,7 +1002,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
   const int column0 = at.tile * S::kColumns, mine0 = column0 + column_wave * 16 * S::CF;
   const int first = at.chunk * parts.chunk_rows, last = min(p.nk, first + parts.chunk_rows);
   const HeadRows keys = head_rows<Tag>(p.k, at.b, kv), values = head_rows<Tag>(p.v, at.b, kv);
-  const Scores<S::kPlain> scores(p, at.head);
+  const Scores<S::kKind> scores(p, at.head);
   const bool masked = p.k_segments != nullptr;
 
   u32x4 q[S::CF][S::kSlices], go[S::CF][S::kSlices];
@@ -1097,7 +1102,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kWavesPerSimd) attn_grad_q_ker
       const f32x2 *points = reinterpret_cast<const f32x2 *>(tile + S::kPoints) + block * 16 + 4 * g;
       const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
       const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
-      form_weights<Tag, S::kPlain, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int, int, int f) { return lse[f]; }, [&] {
+      form_weights<Tag, S::kKind, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int, int, int f) { return lse[f]; }, [&] {
         if (every) return;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -1239,7 +1244,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kGradKvWaves) attn_grad_kv_ker
 
   for (int head = head0; head < head0 + heads_here; ++head) {
     const HeadRows queries = head_rows<Tag>(p.q, at.b, head), grads = head_rows<Tag>(p.grad_out, at.b, head);
-    const Scores<S::kPlain> scores(p, head);
+    const Scores<S::kKind> scores(p, head);
     TileLoads<S> next_q, next_g;
     RowLoads next = {};
     auto request = [&](int row0) {
@@ -1289,7 +1294,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kGradKvWaves) attn_grad_kv_ker
         const int *segments = reinterpret_cast<const int *>(tile + S::kSegments) + block * 16 + 4 * g;
         const float *poison = reinterpret_cast<const float *>(tile + S::kPoison) + block * 16 + 4 * g;
         const float *lse = reinterpret_cast<const float *>(tile + S::kLse) + block * 16 + 4 * g;
-        form_weights<Tag, S::kPlain, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int h, int r, int) { return lse[h * 16 + r]; },
+        form_weights<Tag, S::kKind, S::CF>(scores, s, far, bend, point, [&](int h, int r) { return points[h * 16 + r]; }, [&](int h, int r, int) { return lse[h * 16 + r]; },
                                  [&] {
                                    if (every) return;
 #pragma unroll
@@ -1392,21 +1397,21 @@ Mode column_mode(long long heads, int columns, bool masked, bool even) {
 }
 // Rows of a tile and sixteens of columns a wave, by the bytes of a row: narrow rows make long tiles; a wave with two sixteens reads half as
 // much LDS, but backward it has no room for rows of 256 bytes (the gradients' kernels, 16 heads of 128, 4096 queries, 16 bits: 1560 us for 857).
-template <typename Tag, bool PLAIN, int W>
+template <typename Tag, int KIND, int W>
 struct ForwardModes {
   static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 256 ? 1 : 2;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 256 ? 1 : 2), kTwo, 4> Columns64;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), (kBytes > 128 ? 1 : 2), 4> Columns32;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
+  typedef Shape<Tag, KIND, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
+  typedef Shape<Tag, KIND, W, (kBytes > 128 ? 64 : 128), (kBytes > 256 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, KIND, W, (kBytes > 128 ? 64 : kBytes > 64 ? 128 : 256), (kBytes > 128 ? 2 : 4), (kBytes > 128 ? 1 : 2), 4> Columns32;
+  typedef Shape<Tag, KIND, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
 };
-template <typename Tag, bool PLAIN, int W>
+template <typename Tag, int KIND, int W>
 struct BackwardModes {
   static constexpr int kBytes = W * Tag::kBytes, kTwo = kBytes > 128 ? 1 : 2;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 64 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), kTwo, 4> Columns32;
-  typedef Shape<Tag, PLAIN, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
+  typedef Shape<Tag, KIND, W, (kBytes > 64 ? 64 : 128), 1, kTwo, 4> Columns128;
+  typedef Shape<Tag, KIND, W, (kBytes > 64 ? 64 : 128), (kBytes > 128 ? 1 : 2), kTwo, 4> Columns64;
+  typedef Shape<Tag, KIND, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), kTwo, 4> Columns32;
+  typedef Shape<Tag, KIND, W, (kBytes > 128 ? 64 : 128), (kBytes > 128 ? 2 : 4), 1, 4> Columns16;
 };
 
 template <typename S, typename... A>
@@ -1544,10 +1549,10 @@ hipError_t grad_kv_shape(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
   return hipGetLastError();
 }
 
-template <typename Tag, bool PLAIN, int W>
+template <typename Tag, int KIND, int W>
 hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  typedef ForwardModes<Tag, PLAIN, W> M;
-  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, !PLAIN || W <= 64)) {
+  typedef ForwardModes<Tag, KIND, W> M;
+  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, KIND != kPlainScores || W <= 64)) {
     case kColumns128: return forward_shape<typename M::Columns128>(p, stream, bytes);
     case kColumns64: return forward_shape<typename M::Columns64>(p, stream, bytes);
     case kColumns32: return forward_shape<typename M::Columns32>(p, stream, bytes);
@@ -1555,20 +1560,20 @@ hipError_t forward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes)
   }
 }
 
-template <typename Tag, bool PLAIN, int W>
+template <typename Tag, int KIND, int W>
 hipError_t backward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  typedef BackwardModes<Tag, PLAIN, W> M;
+  typedef BackwardModes<Tag, KIND, W> M;
   const bool keys = bytes != nullptr || p.grad_k != nullptr || p.grad_v != nullptr;
   size_t q_bytes = 0, kv_bytes = 0;
   hipError_t e = hipSuccess;
-  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, !PLAIN || W <= 64)) {
+  switch (column_mode((long long)p.batch * p.heads, p.nq, p.k_segments != nullptr, KIND != kPlainScores || W <= 64)) {
     case kColumns128: e = grad_q_shape<typename M::Columns128>(p, stream, bytes ? &q_bytes : nullptr); break;
     case kColumns64: e = grad_q_shape<typename M::Columns64>(p, stream, bytes ? &q_bytes : nullptr); break;
     case kColumns32: e = grad_q_shape<typename M::Columns32>(p, stream, bytes ? &q_bytes : nullptr); break;
     default: e = grad_q_shape<typename M::Columns16>(p, stream, bytes ? &q_bytes : nullptr);
   }
   if (e != hipSuccess || !keys) return e;
-  switch (column_mode((long long)p.batch * p.kv_heads, p.nk, p.k_segments != nullptr, !PLAIN || W <= 64)) {
+  switch (column_mode((long long)p.batch * p.kv_heads, p.nk, p.k_segments != nullptr, KIND != kPlainScores || W <= 64)) {
     case kColumns128: e = grad_kv_shape<typename M::Columns128>(p, stream, bytes ? &kv_bytes : nullptr); break;
     case kColumns64: e = grad_kv_shape<typename M::Columns64>(p, stream, bytes ? &kv_bytes : nullptr); break;
     case kColumns32: e = grad_kv_shape<typename M::Columns32>(p, stream, bytes ? &kv_bytes : nullptr); break;
@@ -1580,23 +1585,29 @@ hipError_t backward_width(const AttnLaunch &p, hipStream_t stream, size_t *bytes
 
 bool plain_scores(const AttnLaunch &p) { return p.cap == 0.f && p.slopes == nullptr && p.scale > 0.f; }
 
-template <typename Tag, bool PLAIN>
+template <typename Tag, int KIND>
 hipError_t forward_scores(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  if (p.width <= 32) return forward_width<Tag, PLAIN, 32>(p, stream, bytes);
-  return p.width <= 64 ? forward_width<Tag, PLAIN, 64>(p, stream, bytes) : forward_width<Tag, PLAIN, 128>(p, stream, bytes);
+  if (p.width <= 32) return forward_width<Tag, KIND, 32>(p, stream, bytes);
+  return p.width <= 64 ? forward_width<Tag, KIND, 64>(p, stream, bytes) : forward_width<Tag, KIND, 128>(p, stream, bytes);
 }
 template <typename Tag>
 hipError_t forward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  return plain_scores(p) ? forward_scores<Tag, true>(p, stream, bytes) : forward_scores<Tag, false>(p, stream, bytes);
+  if (plain_scores(p)) return forward_scores<Tag, kPlainScores>(p, stream, bytes);
+  if constexpr (Tag::kBytes == 2)
+    if (p.cap > kQuickCap) return forward_scores<Tag, kHighCap>(p, stream, bytes);
+  return forward_scores<Tag, kAnyScores>(p, stream, bytes);
 }
-template <typename Tag, bool PLAIN>
+template <typename Tag, int KIND>
 hipError_t backward_scores(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  if (p.width <= 32) return backward_width<Tag, PLAIN, 32>(p, stream, bytes);
-  return p.width <= 64 ? backward_width<Tag, PLAIN, 64>(p, stream, bytes) : backward_width<Tag, PLAIN, 128>(p, stream, bytes);
+  if (p.width <= 32) return backward_width<Tag, KIND, 32>(p, stream, bytes);
+  return p.width <= 64 ? backward_width<Tag, KIND, 64>(p, stream, bytes) : backward_width<Tag, KIND, 128>(p, stream, bytes);
 }
 template <typename Tag>
 hipError_t backward_t(const AttnLaunch &p, hipStream_t stream, size_t *bytes) {
-  return plain_scores(p) ? backward_scores<Tag, true>(p, stream, bytes) : backward_scores<Tag, false>(p, stream, bytes);
+  if (plain_scores(p)) return backward_scores<Tag, kPlainScores>(p, stream, bytes);
+  if constexpr (Tag::kBytes == 2)
+    if (p.cap > kQuickCap) return backward_scores<Tag, kHighCap>(p, stream, bytes);
+  return backward_scores<Tag, kAnyScores>(p, stream, bytes);
 }
 
 }  // namespace

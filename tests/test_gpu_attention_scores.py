@@ -118,3 +118,12 @@ def test_gradients_of_rows_that_are_far_from_all_keys(cap, lq, lk, dtype):
     assert torch.isnan(grad_query[:, 1:, 1]).all() and torch.isnan(grad_key[:, :, 1]).all() and torch.isnan(grad_value[:, :, 1]).all()
     assert all(torch.isfinite(g).all() for g in (grad_query[:, :, 0], grad_query[:, 0], grad_key[:, :, 0], grad_value[:, :, 0], grad_slopes[0]))
     assert torch.isnan(grad_slopes[1])
+
+
+# heads and queries for every number of columns a workgroup takes
+@pytest.mark.parametrize("dtype", (F16, BF16), ids=IDS.get)
+@pytest.mark.parametrize("n,m,lq,mask,distance", [(1, 2, 200, "none", True), (1, 8, 1030, "random", False), (1, 16, 1030, "none", False), (2, 16, 1030, "none", True),
+                                                  (3, 16, 1030, "none", False), (2, 16, 600, "documents", True)])
+@pytest.mark.parametrize("width", (32, 64, 128))
+def test_large_caps_in_every_shape_of_workgroup(width, n, m, lq, mask, distance, dtype):
+    check(inputs(n, lq, lq, m, m, width, dtype, mask=mask, distance=distance, seed=width + m), device="cuda", cap=1000.0)
